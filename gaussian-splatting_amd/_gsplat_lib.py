@@ -164,6 +164,24 @@ def lib():
     L.gso_compact_map.argtypes = [C.c_int64, _vp, _vp, _vp, C.c_size_t, C.POINTER(C.c_int64), _vp]
     L.gso_gather_rows.restype = C.c_int
     L.gso_gather_rows.argtypes = [_vp, _vp, _vp, C.c_int64, C.c_int, _vp]
+    L.gso_norm_temp_bytes.restype = C.c_size_t
+    L.gso_norm_temp_bytes.argtypes = [C.c_int, _vp]
+    L.gso_grad_norm.restype = C.c_int
+    L.gso_grad_norm.argtypes = [C.c_int, _vp, _vp, _vp, C.c_int, _vp, C.c_size_t, _vp, _vp]
+    L.gso_norm_finish.restype = C.c_int
+    L.gso_norm_finish.argtypes = [_vp, C.c_int, C.c_int, _vp, _vp]
+    L.gso_clip_grads.restype = C.c_int
+    L.gso_clip_grads.argtypes = [C.c_int, _vp, _vp, _vp, C.c_int, C.c_double, _vp, C.c_int, _vp, _vp]
+    L.gso_adam_clipped.restype = C.c_int
+    L.gso_adam_clipped.argtypes = [C.c_int, _vp, _vp, C.c_int, C.c_double, _vp, C.c_int, _vp, _vp]
+    L.gso_accumulate_weights.restype = C.c_int
+    L.gso_accumulate_weights.argtypes = [C.c_int64, _vp, C.c_int, _vp, _vp, C.c_double, _vp]
+    L.gso_evict_temp_bytes.restype = C.c_size_t
+    L.gso_evict_temp_bytes.argtypes = [C.c_int64]
+    L.gso_evict_select.restype = C.c_int
+    L.gso_evict_select.argtypes = [C.c_int64, _vp, C.c_int64, C.c_int64, _vp, _vp, C.c_size_t, _vp]
+    L.gso_gather_rows_multi.restype = C.c_int
+    L.gso_gather_rows_multi.argtypes = [C.c_int, _vp, _vp, C.c_int64, _vp]
     L.gsr_status_string.restype = C.c_char_p
     L.gsr_status_string.argtypes = [C.c_int]
     L.gsr_struct_bytes.restype = C.c_size_t
@@ -184,7 +202,9 @@ EXPORTED = ("gsr_geom_bytes", "gsr_image_bytes", "gsr_binning_bytes", "gsr_backw
             "gss_ssim_backward", "gss_loss_partial_floats", "gss_l1_ssim_loss_forward", "gss_l1_ssim_loss_backward",
             "gss_l1_partial_floats", "gss_l1_loss_forward", "gss_l1_loss_backward",
             "gso_adam_update", "gso_densify_stats", "gso_densify_select", "gso_mark_nonzero", "gso_prune_mask", "gso_split_children", "gso_compact_temp_bytes", "gso_compact_map",
-            "gso_gather_rows", "gsr_status_string", "gsr_struct_bytes")
+            "gso_gather_rows", "gso_norm_temp_bytes", "gso_grad_norm", "gso_norm_finish", "gso_clip_grads",
+            "gso_adam_clipped", "gso_accumulate_weights", "gso_evict_temp_bytes", "gso_evict_select",
+            "gso_gather_rows_multi", "gsr_status_string", "gsr_struct_bytes")
 
 
 NUM_PROFILE_EVENTS = 21

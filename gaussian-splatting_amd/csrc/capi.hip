@@ -651,6 +651,100 @@ int gso_gather_rows(const void* src, void* dst, const uint32_t* src_of_dst, int6
     return hip_status(launch_gather_rows(src, dst, src_of_dst, K, M, (hipStream_t)stream));
 }
 
+static bool norm_args_ok(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type) {
+    if (n < 0 || norm_type < 0 || norm_type > 2) return false;
+    if (n > 0 && (!grads || !numels || !types)) return false;
+    for (int i = 0; i < n; ++i) {
+        if (numels[i] < 0 || types[i] < GSO_F32 || types[i] > GSO_F16) return false;
+        if (numels[i] > 0 && (!grads[i] || ((uintptr_t)grads[i] & (types[i] == GSO_F32 ? 3u : 1u)) != 0)) return false;
+    }
+    return true;
+}
+
+size_t gso_norm_temp_bytes(int n, const int64_t* numels) {
+    if (n < 0 || (n > 0 && !numels)) return 0;
+    return norm_temp_bytes(n, numels);
+}
+
+int gso_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type, void* temp,
+                  size_t temp_bytes, int* partials, void* stream) {
+    if (!partials || !temp || ((uintptr_t)temp & 7u) != 0) return GSR_ERR_ARG;
+    if (!norm_args_ok(n, grads, numels, types, norm_type)) return GSR_ERR_ARG;
+    if (!norm_fits(n, numels)) return GSR_ERR_OVERFLOW;
+    if (temp_bytes < norm_temp_bytes(n, numels)) return GSR_ERR_BUFFER;
+    return hip_status(launch_grad_norm(n, grads, numels, types, norm_type, temp, partials, (hipStream_t)stream));
+}
+
+int gso_norm_finish(void* temp, int partials, int norm_type, float* norm, void* stream) {
+    if (!temp || !norm || partials < 0 || norm_type < 0 || norm_type > 2) return GSR_ERR_ARG;
+    return hip_status(launch_norm_finish(temp, partials, norm_type, 0.0, norm, (hipStream_t)stream));
+}
+
+int gso_clip_grads(int n, void* const* grads, const int64_t* numels, const int* types, int norm_type, double max_norm,
+                   void* temp, int partials, float* norm, void* stream) {
+    if (!temp || !norm || partials < 0 || !(max_norm >= 0.0)) return GSR_ERR_ARG;
+    if (!norm_args_ok(n, (const void* const*)grads, numels, types, norm_type)) return GSR_ERR_ARG;
+    if (!norm_fits(n, numels)) return GSR_ERR_OVERFLOW;
+    return hip_status(launch_clip_grads(n, grads, numels, types, norm_type, max_norm, temp, partials, norm,
+                                        (hipStream_t)stream));
+}
+
+int gso_adam_clipped(int n, const GsoAdamTensor* tensors, const uint8_t* visible, int norm_type, double max_norm,
+                     void* temp, int partials, float* norm, void* stream) {
+    if (n < 0 || (n > 0 && !tensors) || !temp || !norm || partials < 0 || !(max_norm >= 0.0)) return GSR_ERR_ARG;
+    if (norm_type < 0 || norm_type > 2) return GSR_ERR_ARG;
+    for (int i = 0; i < n; ++i) {
+        const GsoAdamTensor& a = tensors[i];
+        if (a.rows < 0 || a.width <= 0) return GSR_ERR_ARG;
+        if (a.rows >= (1ll << 31) || a.width >= (1ll << 31) || a.rows * a.width >= (1ll << 40)) return GSR_ERR_OVERFLOW;
+        if (a.rows == 0) continue;
+        if (!a.param || !a.grad || !a.exp_avg || !a.exp_avg_sq) return GSR_ERR_ARG;
+        if ((((uintptr_t)a.param | (uintptr_t)a.grad | (uintptr_t)a.exp_avg | (uintptr_t)a.exp_avg_sq) & 3u) != 0)
+            return GSR_ERR_ARG;
+        if (!(a.bias_correction1 > 0.0) || !(a.bias_correction2_sqrt > 0.0)) return GSR_ERR_ARG;
+    }
+    return hip_status(launch_adam_clipped(n, tensors, visible, norm_type, max_norm, temp, partials, norm,
+                                          (hipStream_t)stream));
+}
+
+int gso_accumulate_weights(int64_t N, float* weights, int views, const float* const* contributions, const float* opacity,
+                           double decay, void* stream) {
+    if (N < 0 || views < 0) return GSR_ERR_ARG;
+    if (N == 0) return GSR_OK;
+    if (N >= (1ll << 31)) return GSR_ERR_OVERFLOW;
+    if (!weights || (views > 0 && !contributions)) return GSR_ERR_ARG;
+    for (int v = 0; v < views; ++v)
+        if (!contributions[v]) return GSR_ERR_ARG;
+    return hip_status(launch_accumulate_weights(N, weights, views, contributions, opacity, (float)decay,
+                                                (hipStream_t)stream));
+}
+
+size_t gso_evict_temp_bytes(int64_t N) { return evict_temp_bytes(N > 0 ? N : 1); }
+
+int gso_evict_select(int64_t N, const float* weights, int64_t budget, int64_t recent, int32_t* rows, void* temp,
+                     size_t temp_bytes, void* stream) {
+    if (N < 0 || budget < 0 || recent < 0 || recent > budget) return GSR_ERR_ARG;
+    if (N == 0 || budget == 0) return GSR_OK;
+    if (N >= (1ll << 31)) return GSR_ERR_OVERFLOW;
+    if (!weights || !rows || !temp) return GSR_ERR_ARG;
+    if (temp_bytes < evict_temp_bytes(N)) return GSR_ERR_BUFFER;
+    return hip_status(launch_evict_select(N, weights, budget, recent, rows, temp, (hipStream_t)stream));
+}
+
+int gso_gather_rows_multi(int n, const GsoRowCopy* copies, const int32_t* rows, int64_t K, void* stream) {
+    if (n < 0 || K < 0) return GSR_ERR_ARG;
+    if (n == 0 || K == 0) return GSR_OK;
+    if (K >= (1ll << 31)) return GSR_ERR_OVERFLOW;
+    if (!copies || !rows) return GSR_ERR_ARG;
+    for (int i = 0; i < n; ++i) {
+        const GsoRowCopy& c = copies[i];
+        if (c.row_bytes < 0 || c.src_pitch < 0) return GSR_ERR_ARG;
+        if (c.row_bytes >= (1ll << 31) || K * c.row_bytes >= (1ll << 42)) return GSR_ERR_OVERFLOW;
+        if (c.row_bytes > 0 && (!c.src || !c.dst)) return GSR_ERR_ARG;
+    }
+    return hip_status(launch_gather_rows_multi(n, copies, rows, K, (hipStream_t)stream));
+}
+
 const char* gsr_status_string(int status) {
     switch (status) {
         case GSR_OK: return "ok";

@@ -211,6 +211,24 @@ hipError_t launch_compact_map(int64_t N, const uint8_t* keep, uint32_t* src_of_d
 hipError_t launch_gather_rows(const void* src, void* dst, const uint32_t* src_of_dst, int64_t K, int M,
                               hipStream_t st);
 
+// Gradient norm, clipping and the Adam step under a ceiling (grad_clip.hip); kind: 0 max |g|, 1 sum |g|, 2 sqrt(sum g^2).
+bool norm_fits(int n, const int64_t* numels);
+size_t norm_temp_bytes(int n, const int64_t* numels);
+hipError_t launch_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int kind, void* temp,
+                            int* partials, hipStream_t st);
+hipError_t launch_norm_finish(void* temp, int partials, int kind, double max_norm, float* norm, hipStream_t st);
+hipError_t launch_clip_grads(int n, void* const* grads, const int64_t* numels, const int* types, int kind, double max_norm,
+                             void* temp, int partials, float* norm, hipStream_t st);
+hipError_t launch_adam_clipped(int n, const GsoAdamTensor* tensors, const uint8_t* visible, int kind, double max_norm,
+                               void* temp, int partials, float* norm, hipStream_t st);
+// Accumulated weights and eviction (evict.hip).
+hipError_t launch_accumulate_weights(int64_t N, float* weights, int views, const float* const* contributions,
+                                     const float* opacity, float decay, hipStream_t st);
+size_t evict_temp_bytes(int64_t N);
+hipError_t launch_evict_select(int64_t N, const float* weights, int64_t budget, int64_t recent, int32_t* rows, void* temp,
+                               hipStream_t st);
+hipError_t launch_gather_rows_multi(int n, const GsoRowCopy* copies, const int32_t* rows, int64_t K, hipStream_t st);
+
 hipError_t launch_knn(int P, const float* points, float* out, void* temp, hipStream_t st);
 size_t knn_temp_bytes(int P);
 

@@ -242,8 +242,11 @@ torch::Tensor markVisible(const torch::Tensor& means3D, const torch::Tensor& vie
     return present;
 }
 
+void bind_optim(pybind11::module_& m);   // optim_ext.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     namespace py = pybind11;
+    bind_optim(m);
     m.def("rasterize_gaussians", &RasterizeGaussiansHIP, py::arg("background"), py::arg("means3D"), py::arg("colors"),
           py::arg("opacity"), py::arg("scales"), py::arg("rotations"), py::arg("scale_modifier"),
           py::arg("cov3D_precomp"), py::arg("viewmatrix"), py::arg("projmatrix"), py::arg("tan_fovx"),

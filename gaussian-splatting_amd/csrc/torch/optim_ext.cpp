@@ -1,0 +1,284 @@
+// Host layer of the gradient norm, clipping, the Adam step under a ceiling and the eviction to a row budget
+// (grad_clip.hip, evict.hip): lists of tensors are checked and turned into the C ABI's tables here, because a list of
+// several hundred tensors costs Python more than the kernels take.  Host code only.
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "../../../include/gsplat_amd.h"
+
+namespace {
+
+using torch::Tensor;
+
+void check_rc(int rc, const char* what) { TORCH_CHECK(rc == GSR_OK, what, ": ", gsr_status_string(rc), " (", rc, ")"); }
+
+void* stream_on(const c10::Device& dev) {
+    return (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
+}
+
+int norm_kind(double p, const char* what) {
+    TORCH_CHECK(p == 1.0 || p == 2.0 || (std::isinf(p) && p > 0), what, ": norm_type must be 1, 2 or inf, got ", p);
+    return std::isinf(p) ? 0 : (int)p;
+}
+
+int type_of(const Tensor& t, const char* what) {
+    switch (t.scalar_type()) {
+        case torch::kFloat32: return GSO_F32;
+        case torch::kBFloat16: return GSO_BF16;
+        case torch::kFloat16: return GSO_F16;
+        default: TORCH_CHECK(false, what, ": gradients must be float32, bfloat16 or float16, got ", t.scalar_type());
+    }
+    return 0;
+}
+
+// The gradients of a list of parameters as the C ABI takes them.  A gradient whose elements do not fill a block of
+// memory of their own (a slice of something wider) is worked on in a packed copy.
+struct Grads {
+    std::vector<Tensor> own, packed;   // packed[i] is own[i], or the copy
+    std::vector<void*> ptr;
+    std::vector<int64_t> numel;
+    std::vector<int> type;
+    int n() const { return (int)ptr.size(); }
+    const void* const* cptr() const { return (const void* const*)ptr.data(); }
+};
+
+Grads collect(const std::vector<Tensor>& params, const char* what) {
+    Grads g;
+    const size_t n = params.size();
+    g.own.reserve(n);
+    g.packed.reserve(n);
+    g.ptr.reserve(n);
+    g.numel.reserve(n);
+    g.type.reserve(n);
+    for (const Tensor& p : params) {
+        TORCH_CHECK(p.defined(), what, ": expected tensors");
+        const Tensor& t = p.grad();
+        if (!t.defined()) continue;
+        TORCH_CHECK(t.layout() == c10::kStrided, what, ": gradients must be dense, got layout ", t.layout());
+        TORCH_CHECK(t.is_cuda(), what, ": gradients must be GPU tensors (there is no CPU path), got one on ", t.device());
+        TORCH_CHECK(g.own.empty() || t.device() == g.own[0].device(), what, ": gradients must be on one device, got ",
+                    g.own.empty() ? t.device() : g.own[0].device(), " and ", t.device());
+        g.type.push_back(type_of(t, what));
+        g.own.push_back(t);
+        g.packed.push_back(t.is_non_overlapping_and_dense() ? t : t.contiguous());
+        g.ptr.push_back(g.packed.back().data_ptr());
+        g.numel.push_back(g.packed.back().numel());
+    }
+    return g;
+}
+
+// Scaling in place needs every element once: two gradients in the same memory would race.
+void check_disjoint(const Grads& g, const char* what) {
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    spans.reserve(g.own.size());
+    for (size_t i = 0; i < g.own.size(); ++i) {
+        if (!g.packed[i].is_same(g.own[i])) {
+            for (int64_t d = 0; d < g.own[i].dim(); ++d)
+                TORCH_CHECK(g.own[i].stride(d) != 0 || g.own[i].size(d) <= 1, what,
+                            ": a gradient has several elements in one place (an expanded tensor)");
+        } else if (g.numel[i] > 0) {
+            const uintptr_t at = (uintptr_t)g.ptr[i];
+            spans.emplace_back(at, at + (uintptr_t)g.numel[i] * g.own[i].element_size());
+        }
+    }
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        TORCH_CHECK(spans[i].first >= spans[i - 1].second, what,
+                    ": two gradients share memory (is a parameter listed twice?)");
+}
+
+void check_may_wait(const char* what) {
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, what,
+                ": error_if_nonfinite makes the host wait, which a stream capture does not allow");
+}
+
+struct Norm {
+    Tensor temp, value;
+    int partials = 0;
+};
+
+Norm sums_of(const Grads& g, int kind, void* st, const char* what) {
+    Norm r;
+    const auto opt = torch::TensorOptions().device(g.own[0].device());
+    const size_t bytes = gso_norm_temp_bytes(g.n(), g.numel.data());
+    r.temp = torch::empty({(int64_t)bytes}, opt.dtype(torch::kUInt8));
+    r.value = torch::empty({}, opt.dtype(torch::kFloat32));
+    check_rc(gso_grad_norm(g.n(), g.cptr(), g.numel.data(), g.type.data(), kind, r.temp.data_ptr(), bytes, &r.partials, st),
+             what);
+    return r;
+}
+
+void raise_if_nonfinite(Norm& r, int kind, void* st, const char* what) {
+    check_rc(gso_norm_finish(r.temp.data_ptr(), r.partials, kind, r.value.data_ptr<float>(), st), what);
+    TORCH_CHECK(std::isfinite(r.value.item<float>()), what, ": the total norm of the gradients is ", r.value.item<float>(),
+                " (error_if_nonfinite); nothing was changed");
+}
+
+Tensor grad_norm(const std::vector<Tensor>& params, double norm_type) {
+    const char* what = "grad_norm";
+    const int kind = norm_kind(norm_type, what);
+    const Grads g = collect(params, what);
+    if (g.own.empty()) return torch::zeros({});
+    c10::DeviceGuard guard(g.own[0].device());
+    void* st = stream_on(g.own[0].device());
+    Norm r = sums_of(g, kind, st, what);
+    check_rc(gso_norm_finish(r.temp.data_ptr(), r.partials, kind, r.value.data_ptr<float>(), st), what);
+    return r.value;
+}
+
+Tensor clip_grad_norm(const std::vector<Tensor>& params, double max_norm, double norm_type, bool error_if_nonfinite) {
+    const char* what = "clip_grad_norm_";
+    const int kind = norm_kind(norm_type, what);
+    TORCH_CHECK(max_norm >= 0.0, what, ": max_norm must not be negative or NaN, got ", max_norm);
+    const Grads g = collect(params, what);
+    check_disjoint(g, what);
+    if (g.own.empty()) return torch::zeros({});
+    c10::DeviceGuard guard(g.own[0].device());
+    if (error_if_nonfinite) check_may_wait(what);
+    void* st = stream_on(g.own[0].device());
+    Norm r = sums_of(g, kind, st, what);
+    if (error_if_nonfinite) raise_if_nonfinite(r, kind, st, what);
+    check_rc(gso_clip_grads(g.n(), g.ptr.data(), g.numel.data(), g.type.data(), kind, max_norm, r.temp.data_ptr(), r.partials,
+                            r.value.data_ptr<float>(), st),
+             what);
+    for (size_t i = 0; i < g.own.size(); ++i)
+        if (!g.packed[i].is_same(g.own[i])) g.own[i].copy_(g.packed[i]);
+    return r.value;
+}
+
+// Parameters with their moments, step sizes as the optimizer's groups hold them: scalars has six numbers per tensor,
+// (lr, beta1, beta2, eps, 1 - beta1^t, sqrt(1 - beta2^t)).  Tensors marked `idle` count in the norm and are not updated.
+Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>& exp_avg,
+                    const std::vector<Tensor>& exp_avg_sq, const std::vector<double>& scalars, const std::vector<bool>& idle,
+                    const c10::optional<Tensor>& visible, double max_norm, double norm_type, bool error_if_nonfinite) {
+    const char* what = "clipped_adam_step";
+    const int kind = norm_kind(norm_type, what);
+    const Grads g = collect(params, what);
+    const size_t n = params.size();
+    TORCH_CHECK(g.own.size() == n && exp_avg.size() == n && exp_avg_sq.size() == n && scalars.size() == 6 * n &&
+                    idle.size() == n, what, ": inconsistent lists");
+    if (n == 0) return torch::zeros({});
+    const c10::Device dev = g.own[0].device();
+    c10::DeviceGuard guard(dev);
+    if (error_if_nonfinite) check_may_wait(what);
+    std::vector<GsoAdamTensor> table;
+    std::vector<Tensor> keep;
+    table.reserve(n);
+    for (size_t i = 0; i < n; ++i) {
+        if (idle[i] || params[i].numel() == 0) continue;
+        for (const Tensor* t : {&params[i], &exp_avg[i], &exp_avg_sq[i]})
+            TORCH_CHECK(t->device() == dev && t->scalar_type() == torch::kFloat32 && t->is_contiguous() &&
+                            t->sizes() == params[i].sizes(), what,
+                        ": parameters and moments must be contiguous float32 tensors of one shape on the gradients' device");
+        TORCH_CHECK(g.own[i].scalar_type() == torch::kFloat32, what, ": gradients must be float32");
+        keep.push_back(g.own[i].contiguous());
+        GsoAdamTensor a;
+        a.param = params[i].data_ptr<float>();
+        a.grad = keep.back().data_ptr<float>();
+        a.exp_avg = exp_avg[i].data_ptr<float>();
+        a.exp_avg_sq = exp_avg_sq[i].data_ptr<float>();
+        a.rows = params[i].dim() > 0 ? params[i].size(0) : 1;
+        a.width = params[i].numel() / a.rows;
+        const double* s = &scalars[6 * i];
+        a.lr = s[0]; a.beta1 = s[1]; a.beta2 = s[2]; a.eps = s[3]; a.bias_correction1 = s[4]; a.bias_correction2_sqrt = s[5];
+        TORCH_CHECK(!visible || visible->numel() == a.rows, what, ": visibility must have one entry per Gaussian");
+        table.push_back(a);
+    }
+    void* st = stream_on(dev);
+    Norm r = sums_of(g, kind, st, what);
+    if (error_if_nonfinite) raise_if_nonfinite(r, kind, st, what);
+    check_rc(gso_adam_clipped((int)table.size(), table.data(), visible ? (const uint8_t*)visible->data_ptr() : nullptr, kind,
+                              max_norm, r.temp.data_ptr(), r.partials, r.value.data_ptr<float>(), st),
+             what);
+    return r.value;
+}
+
+void accumulate_weights(const Tensor& weights, const std::vector<Tensor>& contributions, const c10::optional<Tensor>& opacity,
+                        double decay) {
+    const char* what = "accumulate_weights";
+    const int64_t N = weights.numel();
+    std::vector<const float*> ptr;
+    std::vector<Tensor> keep;
+    auto take = [&](const Tensor& t, const char* name) {
+        TORCH_CHECK(t.is_cuda() && t.device() == weights.device() && t.scalar_type() == torch::kFloat32 && t.numel() == N &&
+                        t.dim() >= 1 && t.size(0) == N, what, ": ", name, " must be a float32 GPU tensor with one entry per "
+                    "Gaussian (", N, ") on the weights' device, got ", t.sizes(), " ", t.scalar_type(), " on ", t.device());
+        keep.push_back(t.contiguous());
+        return keep.back().data_ptr<float>();
+    };
+    take(weights, "weights");
+    TORCH_CHECK(weights.is_contiguous(), what, ": weights are updated in place and must be contiguous");
+    TORCH_CHECK(std::isfinite(decay), what, ": decay must be finite, got ", decay);
+    for (const Tensor& c : contributions) ptr.push_back(take(c, "a contribution"));
+    const float* o = opacity ? take(*opacity, "opacity") : nullptr;
+    if (N == 0) return;
+    const uintptr_t w0 = (uintptr_t)weights.data_ptr(), w1 = w0 + (uintptr_t)N * 4;
+    for (size_t i = 1; i < keep.size(); ++i)
+        TORCH_CHECK((uintptr_t)keep[i].data_ptr() >= w1 || (uintptr_t)keep[i].data_ptr() + (uintptr_t)N * 4 <= w0, what,
+                    ": weights must not share memory with what is added to them");
+    c10::DeviceGuard guard(weights.device());
+    check_rc(gso_accumulate_weights(N, weights.data_ptr<float>(), (int)ptr.size(), ptr.data(), o, decay,
+                                    stream_on(weights.device())), what);
+}
+
+Tensor evict_select(const Tensor& weights, int64_t budget, int64_t recent) {
+    const char* what = "evict_rows";
+    TORCH_CHECK(weights.is_cuda(), what, ": weights must be a GPU tensor (there is no CPU path)");
+    const int64_t N = weights.numel();
+    TORCH_CHECK(weights.scalar_type() == torch::kFloat32 && weights.dim() >= 1 && weights.size(0) == N, what,
+                ": weights must be float32 with one entry per row, got ", weights.sizes(), " ", weights.scalar_type());
+    TORCH_CHECK(budget >= 0, what, ": budget must not be negative, got ", budget);
+    TORCH_CHECK(recent >= 0 && recent <= budget, what, ": recent must lie between 0 and the budget (", budget, "), got ",
+                recent);
+    c10::DeviceGuard guard(weights.device());
+    const Tensor w = weights.contiguous();
+    Tensor rows = torch::empty({std::min(N, budget)}, w.options().dtype(torch::kInt32));
+    if (rows.numel() == 0) return rows;
+    const size_t bytes = gso_evict_temp_bytes(N);
+    Tensor temp = torch::empty({(int64_t)bytes}, w.options().dtype(torch::kUInt8));
+    check_rc(gso_evict_select(N, w.data_ptr<float>(), budget, recent, rows.data_ptr<int32_t>(), temp.data_ptr(), bytes,
+                              stream_on(w.device())), what);
+    return rows;
+}
+
+std::vector<Tensor> take_rows(const std::vector<Tensor>& tensors, const Tensor& rows, int64_t N) {
+    const char* what = "evict_rows";
+    const int64_t K = rows.numel();
+    std::vector<Tensor> out, keep;
+    std::vector<GsoRowCopy> copies;
+    out.reserve(tensors.size());
+    for (const Tensor& t : tensors) {
+        TORCH_CHECK(t.layout() == c10::kStrided && t.device() == rows.device() && t.dim() >= 1 && t.size(0) == N, what,
+                    ": every tensor needs one row per weight (", N, ") on ", rows.device(), ", got ", t.sizes(), " on ", t.device());
+        // rows that are packed in themselves may lie any distance apart; others are packed first
+        const Tensor s = (K > 0 && t.numel() > 0 && t.select(0, 0).is_contiguous()) ? t : t.contiguous();
+        std::vector<int64_t> shape = s.sizes().vec();
+        shape[0] = K;
+        out.push_back(torch::empty(shape, s.options()));
+        const int64_t row_bytes = t.numel() / std::max<int64_t>(N, 1) * t.element_size();
+        if (K == 0 || row_bytes == 0) continue;
+        keep.push_back(s);
+        copies.push_back({s.data_ptr(), out.back().data_ptr(), row_bytes, (int64_t)(s.stride(0) * s.element_size())});
+    }
+    c10::DeviceGuard guard(rows.device());
+    check_rc(gso_gather_rows_multi((int)copies.size(), copies.data(), rows.data_ptr<int32_t>(), K, stream_on(rows.device())), what);
+    return out;
+}
+
+}  // namespace
+
+void bind_optim(pybind11::module_& m) {
+    namespace py = pybind11;
+    m.def("grad_norm", &grad_norm);
+    m.def("clip_grad_norm", &clip_grad_norm);
+    m.def("clipped_adam", &clipped_adam);
+    m.def("accumulate_weights", &accumulate_weights);
+    m.def("evict_select", &evict_select);
+    m.def("take_rows", &take_rows);
+}

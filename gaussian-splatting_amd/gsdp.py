@@ -201,6 +201,21 @@ def reduce_densify_stats(xyz_gradient_accum, denom, max_radii2D, group=None):
         w.wait()
 
 
+def reduce_weights(weights, group=None):
+    """The blending weights that the ranks accumulated from their own views (`gsplat_optim.accumulate_weights`),
+    summed, as a new tensor: what every rank hands to `gsplat_optim.evict_optimizer`, so that all replicas keep the same
+    rows.  The ranks' own weights stay as they are and can be added to further; the eviction then filters them."""
+    total = weights.clone()
+    if dist.is_initialized() and dist.get_world_size(group) > 1:
+        if dist.get_backend(group) == "gloo" and total.is_cuda:
+            host = total.cpu()
+            dist.all_reduce(host, op=dist.ReduceOp.SUM, group=group)
+            total.copy_(host)
+        else:
+            dist.all_reduce(total, op=dist.ReduceOp.SUM, group=group)
+    return total
+
+
 def run_views(sink, settings_list, loss_of_view, streams=(), reducer=None, chunks=6):
     """The local views of one step through a `ParamGradSink` (raw-parameter rasterizer path):
     `begin_step`, the forward preprocess of all the views in one pass, `loss_of_view(i, settings)`

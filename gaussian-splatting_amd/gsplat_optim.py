@@ -76,6 +76,128 @@ class FusedGaussianAdam(torch.optim.Adam):
                           "adam update")
         return loss
 
+    def clipped_step(self, max_norm, visibility=None, N=None, norm_type=2.0, error_if_nonfinite=False):
+        """`clip_grad_norm_` over all of this optimizer's gradients followed by `step(visibility, N)`, in two passes
+        over the data: see `clipped_adam_step`.  Returns the norm before clipping."""
+        return clipped_adam_step(self, max_norm, visibility, N, norm_type, error_if_nonfinite)
+
+
+# ---------------------------------------------------------------- gradient norm and clipping
+def _host():
+    """The compiled host layer (csrc/torch/optim_ext.cpp)."""
+    from diff_gaussian_rasterization import _C
+    if _C._hip_ext is None:
+        raise ImportError("the PyTorch host extension is missing or was replaced by a library override: build it with "
+                          "`python gaussian-splatting_amd/csrc/torch/build_ext.py` (there is no CPU fallback)")
+    return _C._hip_ext
+
+
+def _tensors(parameters):
+    return [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+
+
+@torch.no_grad()
+def grad_norm(parameters, norm_type=2.0):
+    """The norm of all the gradients of `parameters` (an iterable of tensors, or one) together, as if they were one
+    vector: norm_type 2, 1 or inf.  A 0-d float32 tensor on the gradients' device; the host does not wait for it.
+
+    Parameters without a gradient are left out (without any: a CPU zero, as torch.nn.utils.clip_grad_norm_ gives).
+    Gradients are float32, bfloat16 or float16 GPU tensors of one device, of mixed types and any sizes.  Sums are held
+    in 64 bits and added in a fixed order, so the result does not depend on the run, and replicas that hold the same
+    gradients (after `gsdp.GradReducer`) get the same bits.  A NaN makes the norm NaN."""
+    return _host().grad_norm(_tensors(parameters), float(norm_type))
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_: scales the gradients in place by min(1, max_norm / (norm + 1e-6)) and returns
+    the norm they had (`grad_norm`).  Under the ceiling the gradients are read once and not written.  As there, a
+    norm that is NaN makes every gradient NaN, and an infinite one makes them zero (NaN where they were infinite);
+    with error_if_nonfinite=True the host waits for the norm and a RuntimeError leaves the gradients as they were (not
+    under stream capture).  Two gradients must not share memory.
+
+    With `ParamGradSink(keep_zero_rows=True)`: scaling leaves zero rows zero, so nothing has to be marked, unless the
+    norm is not finite; a caller that goes on after that calls `sink.mark_rows_dirty()`.
+    When an Adam step follows, `clipped_adam_step` does both with fewer bytes."""
+    return _host().clip_grad_norm(_tensors(parameters), float(max_norm), float(norm_type), bool(error_if_nonfinite))
+
+
+@torch.no_grad()
+def clipped_adam_step(optimizer, max_norm, visibility=None, N=None, norm_type=2.0, error_if_nonfinite=False):
+    """`clip_grad_norm_(all parameters of the optimizer, max_norm)` followed by `FusedGaussianAdam.step(visibility, N)`
+    for a torch.optim.Adam (or FusedGaussianAdam): one pass that sums and one that updates every tensor, which
+    applies the coefficient on the fly.  Parameters and moments get the same bits as from the two calls; the `.grad`
+    tensors keep their unclipped values.  Returns the norm before clipping (0-d tensor, not waited for).
+
+    The norm counts every gradient of the optimizer, also those of groups that take no sparse step because their rows
+    are not N.  Needs contiguous float32 GPU parameters and plain Adam groups (no weight decay, amsgrad, maximize,
+    capturable); cannot be captured into a graph (the bias correction is a number of the host).  error_if_nonfinite:
+    the host waits for the norm and a RuntimeError leaves parameters, moments and step counts as they were."""
+    what = "clipped_adam_step"
+    if not isinstance(optimizer, torch.optim.Adam):
+        raise RuntimeError(f"{what} needs a torch.optim.Adam, got {type(optimizer).__name__}")
+    if not float(max_norm) >= 0.0:
+        raise RuntimeError(f"{what}: max_norm must not be negative or NaN, got {max_norm}")
+    vis = None
+    if visibility is not None:
+        vis = visibility.to(torch.uint8) if visibility.dtype not in (torch.uint8, torch.bool) else visibility
+        vis = vis.contiguous()
+    entries, device = [], None
+    for group in optimizer.param_groups:
+        if group["weight_decay"] or group["amsgrad"] or group["maximize"] or group["capturable"] or group["differentiable"]:
+            raise RuntimeError(f"{what}: weight_decay, amsgrad, maximize, capturable and differentiable are not supported")
+        beta1, beta2 = group["betas"]
+        lr, eps = float(group["lr"]), float(group["eps"])
+        for p in group["params"]:
+            if p.grad is None:
+                continue
+            if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
+                raise RuntimeError(f"{what} needs contiguous float32 GPU parameters (there is no CPU path)")
+            if device is None:
+                device = p.device
+            rows = p.shape[0] if p.dim() > 0 else 1
+            idle = False
+            if vis is not None:
+                idle = N is not None and rows != N   # a group that is not per-Gaussian takes no sparse step
+                if not idle and vis.numel() != rows:
+                    raise RuntimeError("visibility must have one entry per Gaussian")
+            entries.append((p, lr, beta1, beta2, eps, idle))
+    if vis is not None and device is not None and vis.device != device:
+        raise RuntimeError(f"{what}: visibility must be on {device}, got {vis.device}")
+    if device is not None:
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{what} cannot be captured into a graph: its bias correction follows the step count, "
+                                   "which lives on the host")
+    params, m, v, scalars, idles, fresh, counts = [], [], [], [], [], [], []
+    for p, lr, beta1, beta2, eps, idle in entries:
+        st = optimizer.state[p]
+        if len(st) == 0:
+            st["step"] = torch.tensor(0.0, dtype=torch.float32)
+            st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            fresh.append(p)
+        params.append(p)
+        m.append(st["exp_avg"])
+        v.append(st["exp_avg_sq"])
+        idles.append(idle)
+        if idle or vis is not None:
+            scalars += (lr, beta1, beta2, eps, 1.0, 1.0)
+        else:
+            t = float(st["step"]) + 1.0
+            counts.append(st)
+            scalars += (lr, beta1, beta2, eps, 1.0 - beta1 ** t, math.sqrt(1.0 - beta2 ** t))
+    try:
+        norm = _host().clipped_adam(params, m, v, scalars, idles, vis, float(max_norm), float(norm_type),
+                                    bool(error_if_nonfinite))
+    except Exception:
+        for p in fresh:
+            del optimizer.state[p]
+        raise
+    for st in counts:
+        st["step"] += 1
+    return norm
+
 
 @torch.no_grad()
 def add_densification_stats(radii, viewspace_grad, xyz_gradient_accum, denom, max_radii2D):
@@ -310,3 +432,73 @@ def densify_and_prune(optimizer, stats, max_grad, min_opacity, extent, max_scree
     new_stats = dict(xyz_gradient_accum=torch.zeros((n, 1), device=dev), denom=torch.zeros((n, 1), device=dev),
                      max_radii2D=torch.zeros((n,), device=dev))
     return optimizable, new_stats, comp(tmp_radii)
+
+
+# ---------------------------------------------------------------- a model within a row budget
+@torch.no_grad()
+def accumulate_weights(weights, contributions, opacity=None, decay=1.0):
+    """Adds what some views say about how much each Gaussian matters, in place and in one pass:
+
+        weights = decay * weights + sigmoid(opacity) * (contributions[0] + contributions[1] + ...)
+
+    `contributions`: a list of [N] tensors, or one: the `gauss_sum` of each rendered view (the transmittance that
+    reached the Gaussian, summed over its pixels); times the opacity it is what the Gaussian could add to the images, as
+    attention weights summed over queries are what a cache entry gave.  `opacity`: the raw opacities ([N] or [N, 1],
+    logits), None for contributions that are weights already.  decay < 1 forgets old views.  All float32 on one
+    GPU.  With several ranks each accumulates its own views: see `gsdp.reduce_weights`."""
+    contributions = [contributions] if isinstance(contributions, torch.Tensor) else list(contributions)
+    _host().accumulate_weights(weights, contributions, opacity, float(decay))
+    return weights
+
+
+@torch.no_grad()
+def evict_rows(weights, budget, recent=0, tensors=()):
+    """Which rows stay when a model of N rows may have only `budget`, and those rows of `tensors`.
+
+    Kept are the last `recent` rows (densification appends new Gaussians at the end: they have had no time to gather
+    weight) and, of the others, the budget - recent of largest weight; of equal weights the lower row index stays, and a
+    NaN goes first.  Returns (rows, kept): `rows` [min(N, budget)] int32, ascending, and `kept[k] = tensors[k][rows]`
+    as new contiguous tensors, for any number of tensors of any type with N rows.  The number of rows is known
+    beforehand, so unlike `RowCompactor` the host never waits.  `weights`: [N] or [N, 1], float32, on the GPU."""
+    host = _host()
+    rows = host.evict_select(weights, int(budget), int(recent))
+    return rows, host.take_rows(list(tensors), rows, weights.numel())
+
+
+@torch.no_grad()
+def evict_optimizer(optimizer, weights, budget, recent=0, stats=None):
+    """`evict_rows` for the whole model: every group's parameter, its optimizer state and the per-Gaussian tensors
+    of the dict `stats` keep the chosen rows, and the state moves to the new nn.Parameter as `prune_optimizer` moves
+    it.  Returns ({group name: new parameter}, rows, new stats).  Nothing is changed if a tensor does not have one row
+    per weight.  A `ParamGradSink` has to be built anew afterwards, as after densification."""
+    N = weights.numel()
+    stats = {} if stats is None else dict(stats)
+    moved = []   # (group, [state keys])
+    tensors = []
+    for group in optimizer.param_groups:
+        if len(group["params"]) != 1 or "name" not in group:
+            raise RuntimeError("evict_optimizer: every group must have a name and hold one per-Gaussian tensor")
+        p = group["params"][0]
+        if p.dim() == 0 or p.shape[0] != N:
+            raise RuntimeError(f"evict_optimizer: group {group.get('name')!r} has shape {tuple(p.shape)}, the weights "
+                               f"have {N} rows")
+        st = optimizer.state.get(p, None)
+        keys = [k for k, t in st.items() if torch.is_tensor(t) and t.shape == p.shape] if st else []
+        moved.append((group, keys))
+        tensors.append(p.data)
+        tensors += [st[k] for k in keys]
+    tensors += list(stats.values())
+    rows, kept = evict_rows(weights, budget, recent, tensors)
+    kept = iter(kept)
+    optimizable = {}
+    for group, keys in moved:
+        p = group["params"][0]
+        new_p = nn.Parameter(next(kept).requires_grad_(True))
+        st = optimizer.state.pop(p, None)
+        for k in keys:
+            st[k] = next(kept)
+        if st is not None:
+            optimizer.state[new_p] = st
+        group["params"][0] = new_p
+        optimizable[group["name"]] = new_p
+    return optimizable, rows, {k: next(kept) for k in stats}

@@ -449,6 +449,66 @@ int gso_compact_map(int64_t N, const uint8_t* keep, uint32_t* src_of_dst, void* 
                     void* stream);
 int gso_gather_rows(const void* src, void* dst, const uint32_t* src_of_dst, int64_t K, int M, void* stream);
 
+/* Global gradient norm over many tensors, clipping, and the Adam step under the ceiling.  No counterpart in the
+ * reference, which never bounds its gradients.
+ *   norm = sqrt(sum g^2) (norm_type 2), sum |g| (1) or max |g| (0) over all elements of all tensors; a NaN anywhere
+ *          makes it NaN.  Sums are held in 64 bits and added in a fixed order: the same bits in every run.
+ *   c    = min(1, max_norm / (norm + 1e-6)), formed in 64 bits from the unrounded norm, rounded once to float32
+ * `grads` are HOST arrays of n device pointers with their element counts and types (GsoType); elements are contiguous,
+ * pointers aligned to an element, a count of zero (pointer ignored) is allowed.  Tensors may be of different types.
+ *   gso_grad_norm: sums into `temp` (device, 8-byte aligned, gso_norm_temp_bytes(n, numels) bytes), *partials =
+ *     how many sums it left there.
+ *   gso_norm_finish: *norm (device, float32) from `temp`.
+ *   gso_clip_grads: the same, then g <- g * c in place, each product rounded once to the tensor's type; with c = 1
+ *     nothing is read or written.  No two tensors may share memory.
+ *   gso_adam_clipped: *norm, then Adam's update of every tensor with the gradient c * g (the product rounded to float32,
+ *     as clipping in place would store it; the gradients keep their values), operation by operation gso_adam_update's.
+ *     `visible`: device bytes, one per row, or NULL; applies to every tensor of the call.
+ * No call waits for the device, and all can be captured into a graph (the bias corrections are then frozen). */
+typedef enum { GSO_F32 = 0, GSO_BF16 = 1, GSO_F16 = 2 } GsoType;
+typedef struct {
+    float* param;          /* device [rows, width], as are the three below */
+    const float* grad;
+    float* exp_avg;
+    float* exp_avg_sq;
+    int64_t rows;
+    int64_t width;
+    double lr, beta1, beta2, eps, bias_correction1, bias_correction2_sqrt;   /* as gso_adam_update takes them */
+} GsoAdamTensor;
+size_t gso_norm_temp_bytes(int n, const int64_t* numels);
+int gso_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type, void* temp,
+                  size_t temp_bytes, int* partials, void* stream);
+int gso_norm_finish(void* temp, int partials, int norm_type, float* norm, void* stream);
+int gso_clip_grads(int n, void* const* grads, const int64_t* numels, const int* types, int norm_type, double max_norm,
+                   void* temp, int partials, float* norm, void* stream);
+int gso_adam_clipped(int n, const GsoAdamTensor* tensors, const uint8_t* visible, int norm_type, double max_norm,
+                     void* temp, int partials, float* norm, void* stream);
+
+/* A model within a row budget: the views' blending weights are accumulated per Gaussian, and the lightest rows go.
+ * No counterpart in the reference, whose model only shrinks by opacity and size (scene/gaussian_model.py:237-247).
+ *   gso_accumulate_weights: weights[i] = decay * weights[i] + s_i * (contributions[0][i] + ... ), in place;
+ *     contributions: HOST array of `views` device pointers to [N] floats (a view's gauss_sum); s_i =
+ *     sigmoid(opacity[i]) of the raw opacities, or 1 when opacity is NULL.
+ *   gso_evict_select: rows (device, min(N, budget) ints) = in ascending order the last `recent` rows (all N when
+ *     recent >= N) and, of the others, the budget - recent of largest weight; of equal weights the lower index is
+ *     kept, -0 equals 0, and a NaN lies below everything.  0 <= recent <= budget, N < 2^31.
+ *     temp: device, gso_evict_temp_bytes(N).
+ *   gso_gather_rows_multi: for each of n tensors dst[r] = src[rows[r]], r < K: rows of row_bytes bytes of any type,
+ *     src_pitch bytes apart in src and packed in dst.  Entries of `rows` must lie in every src.
+ * None waits for the device: the number of kept rows is known beforehand. */
+typedef struct {
+    const void* src;
+    void* dst;
+    int64_t row_bytes;
+    int64_t src_pitch;
+} GsoRowCopy;
+int gso_accumulate_weights(int64_t N, float* weights, int views, const float* const* contributions, const float* opacity,
+                           double decay, void* stream);
+size_t gso_evict_temp_bytes(int64_t N);
+int gso_evict_select(int64_t N, const float* weights, int64_t budget, int64_t recent, int32_t* rows, void* temp,
+                     size_t temp_bytes, void* stream);
+int gso_gather_rows_multi(int n, const GsoRowCopy* copies, const int32_t* rows, int64_t K, void* stream);
+
 /* The four test hooks below are per calling thread: they change the calls made from the thread that set
  * them and nothing else.
  * Test hook: while on, the radix sorts use the 64-bit look-back status words of sorts of 2^30 pairs and more

@@ -1,0 +1,388 @@
+"""The global gradient norm, clipping and the Adam step under a ceiling, against the formulas in 64 bits.
+
+Tolerances, from the roundings: u = 2^-24 is half a step of float32.  The sums are held in 64 bits, so the norm is off
+by its one rounding, u, and n * 2^-53 for n terms.  The coefficient is rounded once (u), the product with a gradient in
+float32 once (u), and to the gradient's type once more (2^-8 for bfloat16, 2^-11 for float16; below the normal range
+half a step of the type's subnormals)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF_STEP = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+SUBNORMAL = {torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+SHAPES = dict(xyz=(3,), f_dc=(1, 3), f_rest=(15, 3), opacity=(1,), scaling=(3,), rotation=(4,), reps=(4,))
+
+
+def _params(grads):
+    out = []
+    for g in grads:
+        p = torch.nn.Parameter(torch.empty(g.shape, dtype=g.dtype, device=g.device))
+        p.grad = g
+        out.append(p)
+    return out
+
+
+def _norm64(grads, p):
+    """The definition, in 64 bits on the CPU."""
+    flat = np.concatenate([g.detach().double().cpu().numpy().ravel() for g in grads] + [np.zeros(0)])
+    if p == 2.0:
+        return math.sqrt(float(np.sum(flat * flat)))
+    if p == 1.0:
+        return float(np.sum(np.abs(flat)))
+    return float(np.max(np.abs(flat))) if flat.size else 0.0
+
+
+def _make(sizes, dtypes, seed=0, scale=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    return [(torch.randn(s, generator=gen) * scale).to(dtypes[k % len(dtypes)]).cuda() for k, s in enumerate(sizes)]
+
+
+LISTS = [[1], [0, 5, 0], [4095, 4096, 4097], [63, 64, 65, 255, 256, 257], [100003], [(1000, 3), (1000, 15, 3), (1000, 1), ()],
+         [(k * 37) % 611 for k in range(300)], [1 << 20, 1, 1048577]]
+TYPES = [[torch.float32], [torch.bfloat16], [torch.float16], [torch.float32, torch.bfloat16, torch.float16]]
+
+
+@pytest.mark.parametrize("norm_type", [2.0, 1.0, math.inf])
+@pytest.mark.parametrize("dtypes", TYPES, ids=["f32", "bf16", "f16", "mixed"])
+@pytest.mark.parametrize("sizes", LISTS, ids=[str(i) for i in range(len(LISTS))])
+def test_norm_and_clip(sizes, dtypes, norm_type):
+    import gsplat_optim as G
+    grads = _make(sizes, dtypes, seed=len(sizes))
+    params = _params(grads)
+    n = sum(g.numel() for g in grads)
+    ref = _norm64(grads, norm_type)
+    before = [g.clone() for g in grads]
+    got = G.grad_norm(params, norm_type)
+    assert got.shape == () and got.dtype == torch.float32 and got.is_cuda
+    tol = U + 4 * n * 2.0 ** -53
+    assert abs(float(got) - ref) <= tol * ref
+    # under the ceiling: nothing moves
+    kept = G.clip_grad_norm_(params, 2.0 * ref + 1.0, norm_type)
+    assert torch.equal(kept, got) and all(torch.equal(a, b) for a, b in zip(grads, before))
+    # over it
+    ceiling = 0.3 * ref
+    kept = G.clip_grad_norm_(params, ceiling, norm_type)
+    assert torch.equal(kept, got)
+    c = min(1.0, ceiling / (ref + 1e-6))
+    for g, b in zip(grads, before):
+        want = b.double() * c
+        bound = want.abs() * (HALF_STEP[g.dtype] + 3 * U) + SUBNORMAL[g.dtype]
+        assert bool(((g.double() - want).abs() <= bound).all())
+
+
+def test_same_bits_as_torch_semantics_for_a_single_tensor_and_generators():
+    import gsplat_optim as G
+    g = _make([1000], [torch.float32])[0]
+    p = _params([g])[0]
+    n = G.grad_norm(p)
+    assert torch.equal(n, G.grad_norm(x for x in [p, torch.nn.Parameter(torch.empty(3, device="cuda"))]))
+    z = G.clip_grad_norm_([torch.nn.Parameter(torch.empty(3, device="cuda"))], 1.0)
+    assert z.shape == () and float(z) == 0.0
+    assert float(G.grad_norm([])) == 0.0
+    q = torch.nn.Parameter(p.detach().clone())
+    q.grad = g.clone()
+    a, b = G.clip_grad_norm_(p, 0.5), torch.nn.utils.clip_grad_norm_(q, 0.5)
+    assert abs(float(a) - float(b)) <= 1e-5 * float(b)
+    assert torch.allclose(p.grad, q.grad, rtol=1e-5, atol=0)
+
+
+@pytest.mark.parametrize("scale", [3e38, 1e-30, 1e-44, 0.0])
+@pytest.mark.parametrize("norm_type", [2.0, 1.0, math.inf])
+def test_extreme_sizes_do_not_overflow_or_vanish(scale, norm_type):
+    import gsplat_optim as G
+    g = torch.full((5001,), scale, device="cuda")
+    if scale == 3e38:
+        g[1:] = 1e36
+    ref = _norm64([g], norm_type)
+    got = float(G.grad_norm(_params([g]), norm_type))
+    if ref > float(np.finfo(np.float32).max):
+        assert got == math.inf
+        ref64 = ref
+    else:
+        assert abs(got - ref) <= ref * (U + 1e-11) + SUBNORMAL[torch.float32]
+        ref64 = ref
+    before = g.clone()
+    G.clip_grad_norm_(_params([g]), 0.25 * ref64 if ref64 < 1e38 else 1e37, norm_type)
+    c = min(1.0, (0.25 * ref64 if ref64 < 1e38 else 1e37) / (ref64 + 1e-6))
+    want = before.double() * c
+    assert bool(((g.double() - want).abs() <= want.abs() * 3 * U + c * 0 + SUBNORMAL[torch.float32] + before.double().abs() * 2.0 ** -150).all())
+
+
+@pytest.mark.parametrize("norm_type", [2.0, 1.0, math.inf])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_nonfinite_gradients(norm_type, bad):
+    import gsplat_optim as G
+    grads = _make([3000, 5000, 17], [torch.float32, torch.bfloat16, torch.float16], seed=2)
+    grads[1][4321] = bad
+    before = [g.clone() for g in grads]
+    with pytest.raises(RuntimeError, match="nothing was changed"):
+        G.clip_grad_norm_(_params(grads), 1.0, norm_type, error_if_nonfinite=True)
+    same = lambda: all(torch.equal(torch.nan_to_num(a.float()), torch.nan_to_num(b.float())) for a, b in zip(grads, before))
+    assert same()
+    n = G.clip_grad_norm_(_params(grads), 1.0, norm_type)
+    if math.isnan(bad):
+        assert math.isnan(float(n)) and all(bool(g.isnan().all()) for g in grads)
+    else:
+        assert math.isinf(float(n)) and float(n) > 0
+        assert bool(grads[1][4321].isnan()) and int(grads[1].isnan().sum()) == 1
+        assert all(float(torch.nan_to_num(g.float(), nan=0.0).abs().max()) == 0.0 for g in grads)
+    # an infinite ceiling never clips
+    h = _make([100], [torch.float32])[0]
+    was = h.clone()
+    G.clip_grad_norm_(_params([h]), math.inf)
+    assert torch.equal(h, was)
+    G.clip_grad_norm_(_params([h]), 0.0)
+    assert float(h.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("offset", [1, 2, 3, 5, 7])
+def test_neighbours_of_a_gradient_are_neither_counted_nor_touched(dtype, offset):
+    """Gradients that start at any element of a wider buffer, next to NaN."""
+    import gsplat_optim as G
+    for n in (1, 2, 7, 8, 9, 4096 - offset, 4096, 4097, 10001):
+        buf = torch.full((n + offset + 9,), math.nan, dtype=dtype, device="cuda")
+        g = buf[offset:offset + n]
+        g.copy_(_make([n], [dtype], seed=n)[0])
+        before = g.clone()
+        ref = _norm64([g], 2.0)
+        got = G.clip_grad_norm_(_params([g]), 0.5 * ref)
+        assert abs(float(got) - ref) <= ref * (U + 1e-11)
+        assert bool(buf[:offset].isnan().all()) and bool(buf[offset + n:].isnan().all())
+        want = before.double() * (0.5 * ref / (ref + 1e-6))
+        assert bool(((g.double() - want).abs() <= want.abs() * (HALF_STEP[dtype] + 3 * U) + SUBNORMAL[dtype]).all())
+
+
+def test_gradients_of_other_layouts():
+    import gsplat_optim as G
+    wide = torch.randn(500, 8, device="cuda")
+    keep = wide.clone()
+    turned = torch.randn(70, 30, device="cuda")
+    sparse = torch.randn(40, 40, device="cuda")
+    grads = [wide[:, 2:5], turned.t(), sparse[::2, ::3]]
+    refs = [g.clone() for g in grads]
+    ref = _norm64(grads, 2.0)
+    params = []
+    for g in grads:
+        p = torch.nn.Parameter(torch.empty(g.shape, device="cuda"))
+        p.grad = g
+        params.append(p)
+    got = G.clip_grad_norm_(params, 0.1)
+    assert abs(float(got) - ref) <= ref * (U + 1e-11)
+    c = 0.1 / (ref + 1e-6)
+    for p, r in zip(params, refs):
+        assert bool(((p.grad.double() - r.double() * c).abs() <= r.double().abs() * c * 3 * U + SUBNORMAL[torch.float32]).all())
+    assert torch.equal(wide[:, :2], keep[:, :2]) and torch.equal(wide[:, 5:], keep[:, 5:])
+
+
+def test_refusals_on_the_gpu():
+    import gsplat_optim as G
+    g = torch.ones(10, device="cuda")
+    a, b = _params([g, g])
+    with pytest.raises(RuntimeError, match="share memory"):
+        G.clip_grad_norm_([a, b], 1.0)
+    c, d = _params([g[:6], g[5:]])
+    with pytest.raises(RuntimeError, match="share memory"):
+        G.clip_grad_norm_([d, c], 1.0)
+    assert float(G.grad_norm([a, a])) == pytest.approx(math.sqrt(20.0))   # only read: counted twice, as torch does
+    e = torch.nn.Parameter(torch.ones(10, device="cuda"))
+    e.grad = torch.ones(1, device="cuda").expand(10)
+    assert float(G.grad_norm(e)) == pytest.approx(math.sqrt(10.0))
+    with pytest.raises(RuntimeError, match="expanded"):
+        G.clip_grad_norm_(e, 1.0)
+    f = _params([torch.ones(3, device="cuda", dtype=torch.float64)])
+    with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
+        G.grad_norm(f)
+    with pytest.raises(RuntimeError, match="norm_type"):
+        G.grad_norm(a, 3.0)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(RuntimeError, match="max_norm"):
+            G.clip_grad_norm_(a, bad)
+    cpu = torch.nn.Parameter(torch.ones(3))
+    cpu.grad = torch.ones(3)
+    with pytest.raises(RuntimeError, match="one device|no CPU path"):
+        G.clip_grad_norm_([a, cpu], 1.0)
+    assert torch.equal(g, torch.ones(10, device="cuda"))
+
+
+def test_more_than_2_31_elements():
+    """Offsets beyond 32 bits: a bfloat16 tensor of 2^31 + 12345 elements, zero but for a few at its ends."""
+    import gsplat_optim as G
+    n = (1 << 31) + 12345
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 1, (1 << 31) - 1, 1 << 31, (1 << 31) + 7, n - 1], device="cuda")
+    g[at] = 3.0
+    p = torch.nn.Parameter(torch.empty(n, dtype=torch.bfloat16, device="cuda"))
+    p.grad = g
+    assert float(G.grad_norm(p)) == float(np.float32(math.sqrt(54.0)))
+    assert float(G.grad_norm(p, 1.0)) == 18.0 and float(G.grad_norm(p, math.inf)) == 3.0
+    G.clip_grad_norm_(p, 6.0, 1.0)     # c = 6 / 18.000001
+    assert bool((g[at].float() == 1.0).all())
+    assert int(torch.count_nonzero(g)) == 6
+
+
+def test_on_a_side_stream_and_in_a_graph():
+    """A captured clip replays on new gradients, with eager calls of the same leaves between the replays."""
+    import gsplat_optim as G
+    grads = _make([4097, 300, 100003], [torch.float32, torch.bfloat16, torch.float32], seed=9)
+    params = _params(grads)
+    source = [g.clone() for g in grads]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for g in grads:
+            g.mul_(2.0)
+        n_side = G.clip_grad_norm_(params, 1.0)
+    torch.cuda.current_stream().wait_stream(side)
+    assert abs(float(n_side) - 2 * _norm64(source, 2.0)) <= 2 * _norm64(source, 2.0) * (U + 1e-9)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = G.clip_grad_norm_(params, 1.0)
+    with pytest.raises(RuntimeError, match="capture"):
+        other = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(other):
+            G.clip_grad_norm_(params, 1.0, error_if_nonfinite=True)
+    for k in range(4):
+        for g, s in zip(grads, source):
+            g.copy_(s * (k + 1))
+        eager_in = [g.clone() for g in grads]
+        eager_params = _params(eager_in)
+        graph.replay()
+        eager = G.clip_grad_norm_(eager_params, 1.0)
+        torch.cuda.synchronize()
+        assert torch.equal(captured, eager)
+        assert all(torch.equal(a, b) for a, b in zip(grads, eager_in))
+
+
+# ------------------------------------------------------------------ Adam under the ceiling
+def _optimizer(N, cls, seed=1, steps=3, extra=False):
+    gen = torch.Generator().manual_seed(seed)
+    groups = [{"params": [torch.nn.Parameter(torch.randn(N, *s, generator=gen).cuda())], "lr": 10.0 ** -(1 + k % 4), "name": n}
+              for k, (n, s) in enumerate(SHAPES.items())]
+    if extra:
+        groups.append({"params": [torch.nn.Parameter(torch.randn(5, 3, 4, generator=gen).cuda())], "lr": 1e-3, "name": "exposure"})
+    opt = cls(groups, lr=0.0, eps=1e-15)
+    for _ in range(steps):
+        _fill(opt, gen)
+        opt.step()
+    _fill(opt, gen)
+    return opt
+
+
+def _fill(opt, gen):
+    for g in opt.param_groups:
+        p = g["params"][0]
+        p.grad = (torch.randn(p.shape, generator=gen) * 10.0 ** float(torch.randint(-4, 1, (1,), generator=gen))).cuda()
+
+
+def _dump(opt):
+    out = []
+    for g in opt.param_groups:
+        p = g["params"][0]
+        st = opt.state[p]
+        out += [p.detach().clone(), st["exp_avg"].clone(), st["exp_avg_sq"].clone(), torch.tensor(float(st["step"])).cuda()]
+    return out
+
+
+@pytest.mark.parametrize("N", [1, 2, 63, 1000, 1365, 4099])
+@pytest.mark.parametrize("sparse", [None, 0.0, 0.3, 1.0])
+@pytest.mark.parametrize("ceiling", [0.01, 1e9])
+def test_clipped_step_is_clip_then_step_bit_for_bit(N, sparse, ceiling):
+    import gsplat_optim as G
+    a, b = (_optimizer(N, G.FusedGaussianAdam, extra=True) for _ in range(2))
+    vis = None if sparse is None else torch.rand(N, device="cuda", generator=torch.Generator(device="cuda").manual_seed(N)) < sparse
+    for norm_type in (2.0, 1.0, math.inf):
+        raw = [g["params"][0].grad.clone() for g in a.param_groups]
+        n1 = G.clip_grad_norm_([g["params"][0] for g in b.param_groups], ceiling, norm_type)
+        b.step(vis, None if vis is None else N)
+        n2 = a.clipped_step(ceiling, vis, None if vis is None else N, norm_type=norm_type)
+        assert torch.equal(n1, n2)
+        assert all(torch.equal(g["params"][0].grad, r) for g, r in zip(a.param_groups, raw))
+        for x, y in zip(_dump(a), _dump(b)):
+            assert torch.equal(x, y)
+        for ga, gb in zip(a.param_groups, b.param_groups):
+            gb["params"][0].grad = ga["params"][0].grad.clone()
+
+
+def test_clipped_step_against_the_formula_in_64_bits():
+    """Every rounding of the update counted (u = 2^-24): the gradient 2u, the first moment 3u of its step and u of
+    itself plus what the gradient brings, the second 8u, the denominator 8u, the update 12u more, the parameter u."""
+    import gsplat_optim as G
+    for cls in (torch.optim.Adam, G.FusedGaussianAdam):
+        opt = _optimizer(777, cls)
+        old = [x.double().cpu().numpy() for x in _dump(opt)]
+        grads = [g["params"][0].grad for g in opt.param_groups]
+        ref = _norm64(grads, 2.0)
+        c = 0.05 / (ref + 1e-6)
+        n = G.clipped_adam_step(opt, 0.05)
+        assert abs(float(n) - ref) <= ref * (U + 1e-11)
+        new = [x.double().cpu().numpy() for x in _dump(opt)]
+        for k, group in enumerate(opt.param_groups):
+            p, m, v, t = old[4 * k:4 * k + 4]
+            p1, m1, v1, t1 = new[4 * k:4 * k + 4]
+            t = float(t) + 1
+            assert float(t1) == t
+            g = grads[k].double().cpu().numpy() * c
+            rm = m + 0.1 * (g - m)
+            em = 1.01 * U * (0.1 * (3 * np.abs(g - m) + 2 * np.abs(g)) + np.abs(rm))
+            rv = 0.999 * v + 0.001 * g * g
+            b1, b2 = 1 - 0.9 ** t, 1 - 0.999 ** t
+            den = np.sqrt(rv / b2) + 1e-15
+            step = group["lr"] / b1
+            upd = step * rm / den
+            assert np.all(np.abs(m1 - rm) <= em + 1e-45)
+            assert np.all(np.abs(v1 - rv) <= 8.1 * U * rv + 1e-45)
+            assert np.all(np.abs(p1 - (p - upd)) <= step * em / den * 1.01 + 20 * U * np.abs(upd) + 1.01 * U * np.abs(p - upd))
+
+
+def test_first_step_creates_the_state_and_a_failure_leaves_none():
+    import gsplat_optim as G
+    p = torch.nn.Parameter(torch.ones(100, 3, device="cuda"))
+    opt = G.FusedGaussianAdam([{"params": [p], "lr": 0.1, "name": "xyz"}], eps=1e-15)
+    assert float(opt.clipped_step(1.0)) == 0.0 and len(opt.state) == 0      # no gradient at all: nothing happens
+    p.grad = torch.full((100, 3), math.nan, device="cuda")
+    with pytest.raises(RuntimeError, match="nothing was changed"):
+        opt.clipped_step(1.0, error_if_nonfinite=True)
+    assert len(opt.state) == 0 and torch.equal(p.detach(), torch.ones(100, 3, device="cuda"))
+    p.grad = torch.full((100, 3), 0.5, device="cuda")
+    opt.clipped_step(1.0, error_if_nonfinite=True)
+    assert float(opt.state[p]["step"]) == 1.0
+    assert torch.allclose(p.detach(), torch.full((100, 3), 0.9, device="cuda"), rtol=1e-6)   # 1 - lr * sign(g)
+
+
+def test_clipped_step_refusals():
+    import gsplat_optim as G
+    p = torch.nn.Parameter(torch.ones(10, 3, device="cuda"))
+    p.grad = torch.ones_like(p)
+    for kw in (dict(weight_decay=0.1), dict(amsgrad=True), dict(maximize=True), dict(capturable=True)):
+        with pytest.raises(RuntimeError, match="not supported"):
+            G.clipped_adam_step(torch.optim.Adam([p], lr=1e-3, **kw), 1.0)
+    with pytest.raises(RuntimeError, match="torch.optim.Adam"):
+        G.clipped_adam_step(torch.optim.SGD([p], lr=1e-3), 1.0)
+    opt = G.FusedGaussianAdam([p], lr=1e-3)
+    with pytest.raises(RuntimeError, match="one entry per Gaussian"):
+        opt.clipped_step(1.0, torch.ones(9, dtype=torch.bool, device="cuda"))
+    with pytest.raises(RuntimeError, match="visibility must be on"):
+        opt.clipped_step(1.0, torch.ones(10, dtype=torch.bool))
+    for bad in (-1.0, math.nan):
+        with pytest.raises(RuntimeError, match="max_norm"):
+            opt.clipped_step(bad)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            opt.clipped_step(1.0)
+    assert len(opt.state) == 0 and torch.equal(p.detach(), torch.ones(10, 3, device="cuda"))
+
+
+def test_the_norm_is_the_same_bits_in_every_run():
+    import gsplat_optim as G
+    grads = _make([3_000_001, 77, 500_000], [torch.float32, torch.bfloat16, torch.float16], seed=4)
+    params = _params(grads)
+    first = G.grad_norm(params)
+    for _ in range(20):
+        assert torch.equal(first, G.grad_norm(params))
