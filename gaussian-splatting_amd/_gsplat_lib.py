@@ -165,9 +165,9 @@ def lib():
     L.gso_gather_rows.restype = C.c_int
     L.gso_gather_rows.argtypes = [_vp, _vp, _vp, C.c_int64, C.c_int, _vp]
     L.gso_norm_temp_bytes.restype = C.c_size_t
-    L.gso_norm_temp_bytes.argtypes = [C.c_int, _vp]
+    L.gso_norm_temp_bytes.argtypes = [C.c_int]
     L.gso_grad_norm.restype = C.c_int
-    L.gso_grad_norm.argtypes = [C.c_int, _vp, _vp, _vp, C.c_int, _vp, C.c_size_t, _vp, _vp]
+    L.gso_grad_norm.argtypes = [C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_size_t, _vp, _vp]
     L.gso_norm_finish.restype = C.c_int
     L.gso_norm_finish.argtypes = [_vp, C.c_int, C.c_int, _vp, _vp]
     L.gso_clip_grads.restype = C.c_int

@@ -661,18 +661,16 @@ static bool norm_args_ok(int n, const void* const* grads, const int64_t* numels,
     return true;
 }
 
-size_t gso_norm_temp_bytes(int n, const int64_t* numels) {
-    if (n < 0 || (n > 0 && !numels)) return 0;
-    return norm_temp_bytes(n, numels);
-}
+size_t gso_norm_temp_bytes(int n) { return n < 0 ? 0 : norm_temp_bytes(n); }
 
-int gso_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type, void* temp,
-                  size_t temp_bytes, int* partials, void* stream) {
+int gso_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type, int read_again,
+                  void* temp, size_t temp_bytes, int* partials, void* stream) {
     if (!partials || !temp || ((uintptr_t)temp & 7u) != 0) return GSR_ERR_ARG;
     if (!norm_args_ok(n, grads, numels, types, norm_type)) return GSR_ERR_ARG;
     if (!norm_fits(n, numels)) return GSR_ERR_OVERFLOW;
-    if (temp_bytes < norm_temp_bytes(n, numels)) return GSR_ERR_BUFFER;
-    return hip_status(launch_grad_norm(n, grads, numels, types, norm_type, temp, partials, (hipStream_t)stream));
+    if (temp_bytes < norm_temp_bytes(n)) return GSR_ERR_BUFFER;
+    return hip_status(launch_grad_norm(n, grads, numels, types, norm_type, read_again != 0, temp, partials,
+                                       (hipStream_t)stream));
 }
 
 int gso_norm_finish(void* temp, int partials, int norm_type, float* norm, void* stream) {
@@ -726,7 +724,7 @@ int gso_evict_select(int64_t N, const float* weights, int64_t budget, int64_t re
     if (N < 0 || budget < 0 || recent < 0 || recent > budget) return GSR_ERR_ARG;
     if (N == 0 || budget == 0) return GSR_OK;
     if (N >= (1ll << 31)) return GSR_ERR_OVERFLOW;
-    if (!weights || !rows || !temp) return GSR_ERR_ARG;
+    if (!weights || !rows || !temp || ((uintptr_t)temp & 7u) != 0) return GSR_ERR_ARG;
     if (temp_bytes < evict_temp_bytes(N)) return GSR_ERR_BUFFER;
     return hip_status(launch_evict_select(N, weights, budget, recent, rows, temp, (hipStream_t)stream));
 }

@@ -29,24 +29,56 @@ struct WeightArgs {
     int views;
 };
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Four Gaussians a thread where every pointer allows 16-byte accesses.  Eight views' loads are issued before the first
+// of them is added.
+template <int VEC>
 __global__ void __launch_bounds__(256) accumulate_weights_kernel(const WeightArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    typedef float vec __attribute__((ext_vector_type(VEC)));
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
     if (i >= a.N) return;
-    float s = 0.0f;
-    for (int v = 0; v < a.views; ++v) s += a.contribution[v][i];
-    if (a.opacity) s /= 1.0f + expf(-a.opacity[i]);
-    a.weights[i] = a.weights[i] * a.decay + s;
+    if (VEC > 1 && i + VEC > a.N) {   // the last one to three
+        for (int64_t j = i; j < a.N; ++j) {
+            float s = 0.0f;
+            for (int v = 0; v < a.views; ++v) s += a.contribution[v][j];
+            if (a.opacity) s /= 1.0f + expf(-a.opacity[j]);
+            a.weights[j] = a.weights[j] * a.decay + s;
+        }
+        return;
+    }
+    vec w = *reinterpret_cast<const vec*>(a.weights + i), o = 0.0f, s = 0.0f;
+    if (a.opacity) o = *reinterpret_cast<const vec*>(a.opacity + i);
+    int v = 0;
+    for (; v + 8 <= a.views; v += 8) {
+        vec c[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) c[u] = *reinterpret_cast<const vec*>(a.contribution[v + u] + i);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += c[u];
+    }
+    for (; v < a.views; ++v) s += *reinterpret_cast<const vec*>(a.contribution[v] + i);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        if (a.opacity) s[j] /= 1.0f + expf(-o[j]);
+        w[j] = w[j] * a.decay + s[j];
+    }
+    *reinterpret_cast<vec*>(a.weights + i) = w;
 }
 
 // ------------------------------------------------------------------ selection
 constexpr int HIST_BINS = 2048;
+constexpr int HIST_THREADS = 1024;
+constexpr int HIST_GROUPS = 512;        // two workgroups per CU: each adds its whole histogram to the global one once
+constexpr int HIST_STEP = 4 * HIST_THREADS;
 constexpr int SELECT_THREADS = 256;
-constexpr int SELECT_ROWS = 4096;   // rows of one workgroup
+constexpr int SELECT_ROWS = 4096;       // rows of a tile: sixteen a thread
+constexpr int SELECT_GROUPS = 2048;     // workgroups of the counting and writing kernels, a run of tiles each
 
 struct SelectState {
     uint32_t hist[3][HIST_BINS];
-    uint32_t key;     // the bits of the threshold found so far
-    uint32_t need;    // how many rows that equal them are still to be kept
+    uint2 at[4];      // before each pass, and after the last: the bits of the threshold found so far, and how many rows
+                      // that equal them are still to be kept
 };
 
 // Unsigned integers that order as the weights do: NaN lowest, then -inf .. +inf, and -0 equal to +0.
@@ -58,54 +90,100 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 __global__ void __launch_bounds__(256) select_clear_kernel(SelectState* __restrict__ s, uint32_t need) {
     for (int i = blockIdx.x * 256 + threadIdx.x; i < 3 * HIST_BINS; i += gridDim.x * 256) (&s->hist[0][0])[i] = 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        s->key = 0;
-        s->need = need;
-    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) s->at[0] = make_uint2(0u, need);
 }
 
-__device__ __forceinline__ int pass_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
-__device__ __forceinline__ int pass_bits(int pass) { return pass == 2 ? 10 : 11; }
+constexpr int pass_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+constexpr int pass_bits(int pass) { return pass == 2 ? 10 : 11; }
 
-__global__ void __launch_bounds__(SELECT_THREADS) select_hist_kernel(int64_t old, const float* __restrict__ weights,
-                                                                     SelectState* __restrict__ s, int pass) {
-    __shared__ uint32_t h[HIST_BINS];
-    for (int b = threadIdx.x; b < HIST_BINS; b += SELECT_THREADS) h[b] = 0;
-    __syncthreads();
-    const uint32_t prefix = s->key;
-    const int shift = pass_shift(pass), bits = pass_bits(pass);
-    const int64_t begin = (int64_t)blockIdx.x * SELECT_ROWS;
-    const int64_t end = begin + SELECT_ROWS < old ? begin + SELECT_ROWS : old;
-    for (int64_t i = begin + threadIdx.x; i < end; i += SELECT_THREADS) {
-        const uint32_t k = weight_key(weights[i]);
-        if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&h[(k >> shift) & ((1u << bits) - 1)], 1u);
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {   // inclusive
+#pragma unroll
+    for (int d = 1; d < WAVE; d <<= 1) {
+        const uint32_t o = (uint32_t)__shfl_up((int)v, d, WAVE);
+        if ((int)(threadIdx.x & 63) >= d) v += o;
     }
-    __syncthreads();
-    for (int b = threadIdx.x; b < HIST_BINS; b += SELECT_THREADS)
-        if (h[b]) atomicAdd(&s->hist[pass][b], h[b]);
+    return v;
 }
 
-// The bin that holds the need-th largest key, and how many of it are needed.
-__global__ void __launch_bounds__(256) select_bin_kernel(SelectState* __restrict__ s, int pass) {
-    __shared__ uint32_t sums[256];
-    const uint32_t need = s->need;
-    uint32_t c[8], own = 0;
-    for (int j = 0; j < 8; ++j) {   // thread 0 has the highest bins
-        c[j] = s->hist[pass][HIST_BINS - 1 - (threadIdx.x * 8 + j)];
+// The bin of pass PASS that holds the need-th largest key, and how many of it are needed: every workgroup finds it for
+// itself from the finished histogram, which saves a launch between the passes.
+template <int PASS, int THREADS>
+__device__ __forceinline__ uint2 find_bin(const SelectState* __restrict__ s) {
+    constexpr int PER = HIST_BINS / THREADS;
+    __shared__ uint32_t s_w[THREADS / WAVE];
+    __shared__ uint2 s_found;
+    const uint2 at = s->at[PASS];
+    uint32_t c[PER], own = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {   // thread 0 has the highest bins
+        c[j] = s->hist[PASS][HIST_BINS - 1 - ((int)threadIdx.x * PER + j)];
         own += c[j];
     }
-    sums[threadIdx.x] = own;
+    const uint32_t incl = wave_scan_u32(own);
+    if ((threadIdx.x & 63) == 63) s_w[threadIdx.x >> 6] = incl;
     __syncthreads();
-    uint32_t above = 0;
-    for (int i = 0; i < (int)threadIdx.x; ++i) above += sums[i];
-    __syncthreads();
-    for (int j = 0; j < 8; ++j) {
-        if (above < need && need <= above + c[j]) {
-            s->key = (s->key << pass_bits(pass)) | (uint32_t)(HIST_BINS - 1 - (threadIdx.x * 8 + j));
-            s->need = need - above;
-        }
+    uint32_t above = incl - own;
+    for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) above += s_w[w];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        if (above < at.y && at.y <= above + c[j])
+            s_found = make_uint2((at.x << pass_bits(PASS)) | (uint32_t)(HIST_BINS - 1 - ((int)threadIdx.x * PER + j)), at.y - above);
         above += c[j];
     }
+    __syncthreads();
+    return s_found;
+}
+
+// Adds one to a bin for each lane that is `in`.  Weights repeat (rows that no view has seen are all zero): the lanes
+// that share the first active lane's bin are counted with one ballot and added at once, the others one by one.
+__device__ __forceinline__ void hist_add(uint32_t* h, uint32_t bin, bool in) {
+    const uint64_t act = __ballot(in);
+    if (act == 0) return;
+    const int leader = __builtin_ctzll(act);
+    const uint32_t common = (uint32_t)__builtin_amdgcn_readlane((int)bin, leader);
+    const bool same = in && bin == common;
+    const uint64_t m = __ballot(same);
+    if ((int)(threadIdx.x & 63) == leader) atomicAdd(&h[common], (uint32_t)__popcll(m));
+    else if (in && !same) atomicAdd(&h[bin], 1u);
+}
+
+template <int PASS>
+__global__ void __launch_bounds__(HIST_THREADS) select_hist_kernel(int64_t old, const float* __restrict__ weights,
+                                                                   SelectState* __restrict__ s) {
+    __shared__ uint32_t h[HIST_BINS];
+    constexpr int shift = pass_shift(PASS), bits = pass_bits(PASS);
+    for (int b = threadIdx.x; b < HIST_BINS; b += HIST_THREADS) h[b] = 0;
+    uint32_t prefix = 0;
+    if (PASS > 0) {
+        const uint2 at = find_bin<(PASS > 0 ? PASS - 1 : 0), HIST_THREADS>(s);
+        prefix = at.x;
+        if (blockIdx.x == 0 && threadIdx.x == 0) s->at[PASS] = at;
+    } else {
+        __syncthreads();
+    }
+    const bool aligned = ((uintptr_t)weights & 15) == 0;
+    for (int64_t base = (int64_t)blockIdx.x * HIST_STEP; base < old; base += (int64_t)gridDim.x * HIST_STEP) {
+        const int64_t i = base + 4 * (int)threadIdx.x;
+        float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (aligned && i + 4 <= old) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(weights + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = x[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i + j < old) w[j] = weights[i + j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t k = weight_key(w[j]);
+            const bool in = i + j < old && (PASS == 0 || (uint32_t)((uint64_t)k >> (shift + bits)) == prefix);
+            hist_add(h, (k >> shift) & ((1u << bits) - 1), in);
+        }
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < HIST_BINS; b += HIST_THREADS)
+        if (h[b]) atomicAdd(&s->hist[PASS][b], h[b]);
 }
 
 __device__ __forceinline__ uint32_t block_sum_u32(uint32_t v, uint32_t* s_w) {
@@ -117,34 +195,69 @@ __device__ __forceinline__ uint32_t block_sum_u32(uint32_t v, uint32_t* s_w) {
     return s_w[0] + s_w[1] + s_w[2] + s_w[3];
 }
 
-// Per workgroup: rows above the threshold (the recent ones among them) and rows that equal it.
-__global__ void __launch_bounds__(SELECT_THREADS) select_count_kernel(int64_t N, int64_t old,
+// Sixteen rows of a thread, one bit each: above the threshold (the recent rows among them), and equal to it.
+struct RowBits {
+    uint32_t above, level;
+};
+__device__ __forceinline__ RowBits row_bits(int64_t i, int64_t N, int64_t old, const float* __restrict__ weights, uint32_t key,
+                                            bool aligned) {
+    RowBits r = {0, 0};
+    if (aligned && i + 16 <= old) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(weights + i + 4 * q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t k = weight_key(x[j]);
+                r.above |= (k > key ? 1u : 0u) << (4 * q + j);
+                r.level |= (k == key ? 1u : 0u) << (4 * q + j);
+            }
+        }
+    } else {
+        for (int j = 0; j < 16 && i + j < N; ++j) {
+            if (i + j >= old) {
+                r.above |= 1u << j;
+            } else {
+                const uint32_t k = weight_key(weights[i + j]);
+                r.above |= (k > key ? 1u : 0u) << j;
+                r.level |= (k == key ? 1u : 0u) << j;
+            }
+        }
+    }
+    return r;
+}
+
+// Per workgroup, a run of `tiles` tiles: rows above the threshold and rows that equal it.
+__global__ void __launch_bounds__(SELECT_THREADS) select_count_kernel(int64_t N, int64_t old, int tiles,
                                                                       const float* __restrict__ weights,
-                                                                      const SelectState* __restrict__ s,
-                                                                      uint2* __restrict__ counts) {
+                                                                      SelectState* __restrict__ s, uint2* __restrict__ counts) {
     __shared__ uint32_t s_w[4];
-    const uint32_t key = s->key;
+    const uint2 at = find_bin<2, SELECT_THREADS>(s);
+    if (blockIdx.x == 0 && threadIdx.x == 0) s->at[3] = at;
+    const bool aligned = ((uintptr_t)weights & 15) == 0;
     uint32_t above = 0, level = 0;
-    for (int j = 0; j < SELECT_ROWS / SELECT_THREADS; ++j) {
-        const int64_t i = (int64_t)blockIdx.x * SELECT_ROWS + j * SELECT_THREADS + threadIdx.x;
+    for (int t = 0; t < tiles; ++t) {
+        const int64_t i = ((int64_t)blockIdx.x * tiles + t) * SELECT_ROWS + 16 * (int)threadIdx.x;
         if (i >= N) break;
-        const uint32_t k = i < old ? weight_key(weights[i]) : 0u;
-        above += (i >= old || k > key) ? 1u : 0u;
-        level += (i < old && k == key) ? 1u : 0u;
+        const RowBits r = row_bits(i, N, old, weights, at.x, aligned);
+        above += (uint32_t)__popc(r.above);
+        level += (uint32_t)__popc(r.level);
     }
     above = block_sum_u32(above, s_w);
     level = block_sum_u32(level, s_w);
     if (threadIdx.x == 0) counts[blockIdx.x] = make_uint2(above, level);
 }
 
-__global__ void __launch_bounds__(SELECT_THREADS) select_write_kernel(int64_t N, int64_t old,
+// The kept rows of a tile are gathered in LDS and leave in one run: a thread's own sixteen would be stored 64 bytes apart.
+__global__ void __launch_bounds__(SELECT_THREADS) select_write_kernel(int64_t N, int64_t old, int tiles,
                                                                       const float* __restrict__ weights,
                                                                       const SelectState* __restrict__ s,
                                                                       const uint2* __restrict__ counts,
                                                                       int32_t* __restrict__ rows) {
     __shared__ uint32_t s_w[4];
-    __shared__ uint32_t s_a[4], s_l[4];
-    const uint32_t key = s->key, need = s->need;
+    __shared__ uint32_t s_scan[4];
+    __shared__ int32_t s_rows[SELECT_ROWS];
+    const uint32_t key = s->at[3].x, need = s->at[3].y;
     uint32_t above = 0, level = 0;   // rows of the workgroups before this one
     for (uint32_t b = threadIdx.x; b < blockIdx.x; b += SELECT_THREADS) {
         above += counts[b].x;
@@ -152,29 +265,42 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_write_kernel(int64_t N,
     }
     above = block_sum_u32(above, s_w);
     level = block_sum_u32(level, s_w);
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const uint64_t below = (1ull << lane) - 1;
-    for (int j = 0; j < SELECT_ROWS / SELECT_THREADS; ++j) {
-        const int64_t i = (int64_t)blockIdx.x * SELECT_ROWS + j * SELECT_THREADS + threadIdx.x;
-        const uint32_t k = i < old ? weight_key(weights[i]) : 0u;
-        const bool a = i < N && (i >= old || k > key), l = i < old && k == key;
-        const uint64_t ma = __ballot(a), ml = __ballot(l);
+    const bool aligned = ((uintptr_t)weights & 15) == 0;
+    const int w = threadIdx.x >> 6;
+    for (int t = 0; t < tiles; ++t) {
+        const int64_t tile = ((int64_t)blockIdx.x * tiles + t) * SELECT_ROWS;
+        if (tile >= N) break;
+        const int64_t i = tile + 16 * (int)threadIdx.x;
+        RowBits r = {0, 0};
+        if (i < N) r = row_bits(i, N, old, weights, key, aligned);
+        // both counts of a tile fit 16 bits
+        const uint32_t own = (uint32_t)__popc(r.above) | (uint32_t)__popc(r.level) << 16;
+        const uint32_t incl = wave_scan_u32(own);
+        if ((threadIdx.x & 63) == 63) s_scan[w] = incl;
         __syncthreads();
-        if (lane == 0) {
-            s_a[w] = (uint32_t)__popcll(ma);
-            s_l[w] = (uint32_t)__popcll(ml);
+        uint32_t before = incl - own;
+        for (int x = 0; x < w; ++x) before += s_scan[x];
+        const uint32_t tile_all = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+        uint32_t pl = level + (before >> 16);                       // rows at the threshold before this thread's
+        const uint32_t level_at = level < need ? level : need;      // of them kept before the tile
+        uint32_t out = (before & 0xffffu) + (pl < need ? pl : need) - level_at;
+        const uint32_t any = r.above | r.level;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            if (any >> j & 1u) {
+                const bool l = r.level >> j & 1u;
+                if (!l || pl < need) s_rows[out++] = (int32_t)(i + j);
+                pl += l ? 1u : 0u;
+            }
         }
         __syncthreads();
-        uint32_t pa = above, pl = level;
-        for (int x = 0; x < w; ++x) {
-            pa += s_a[x];
-            pl += s_l[x];
-        }
-        pa += (uint32_t)__popcll(ma & below);
-        pl += (uint32_t)__popcll(ml & below);
-        if (a || (l && pl < need)) rows[pa + (pl < need ? pl : need)] = (int32_t)i;
-        above += s_a[0] + s_a[1] + s_a[2] + s_a[3];
-        level += s_l[0] + s_l[1] + s_l[2] + s_l[3];
+        const uint32_t level_end = level + (tile_all >> 16);
+        const uint32_t kept = (tile_all & 0xffffu) + (level_end < need ? level_end : need) - level_at;
+        const uint32_t to = above + level_at;
+        for (uint32_t x = threadIdx.x; x < kept; x += SELECT_THREADS) rows[to + x] = s_rows[x];
+        above += tile_all & 0xffffu;
+        level = level_end;
+        __syncthreads();
     }
 }
 
@@ -184,36 +310,101 @@ __global__ void __launch_bounds__(256) select_tail_kernel(int64_t first, int64_t
 }
 
 // ------------------------------------------------------------------ rows of many tensors
-constexpr int ROWS_TABLE = 96;   // tensors per launch
-constexpr int64_t ROWS_CHUNK = 4096;   // units of one workgroup
+// A row is cut into the widest units that every address is a multiple of: 16, 8, 4, 2 or 1 bytes.  A workgroup copies a
+// run of rows; a run starts at a multiple of sixteen bytes of the copy.
+constexpr int ROWS_TABLE = 96;              // tensors per launch
+constexpr int ROWS_BYTES = 16384;           // bytes of a workgroup, about
 struct RowsTable {
     const void* src[ROWS_TABLE];
     void* dst[ROWS_TABLE];
     int64_t pitch[ROWS_TABLE];           // bytes between source rows
     uint32_t units[ROWS_TABLE];          // units of a row
-    uint32_t first[ROWS_TABLE + 1];      // first chunk of each tensor
-    uint8_t unit_shift[ROWS_TABLE];      // a unit is 1 << unit_shift bytes: 4, 2 or 1
+    uint32_t first[ROWS_TABLE];          // first workgroup of each tensor
+    uint8_t unit_shift[ROWS_TABLE];      // a unit is 1 << unit_shift bytes
     int n;
 };
 
+// Rows of a workgroup: a multiple of sixteen.
+__host__ __device__ inline uint32_t rows_per_group(uint32_t units, int unit_shift) {
+    const uint64_t row_bytes = (uint64_t)units << unit_shift;
+    const uint32_t r = (uint32_t)(ROWS_BYTES / (row_bytes < ROWS_BYTES ? row_bytes : (uint64_t)ROWS_BYTES));
+    return r < 16 ? 16u : r & ~15u;
+}
+
+// Where unit x of a run of rows lies in the source.
+struct RowSource {
+    const char* src;
+    int64_t pitch;
+    const int32_t* rows;
+    uint32_t M, magic;
+    // x < 2^32, and M = 1 or a multiplier for M
+    __device__ __forceinline__ uint32_t row(uint32_t x) const { return M == 1 ? x : (uint32_t)(((uint64_t)x * magic) >> 32); }
+    __device__ __forceinline__ const char* at(uint32_t r) const { return src + (int64_t)rows[r] * pitch; }
+};
+
+template <typename T>
+__device__ __forceinline__ void copy_units(const RowSource& s, T* __restrict__ dst, uint64_t total) {
+    if (s.magic || s.M == 1) {
+        for (uint32_t x = threadIdx.x; x < (uint32_t)total; x += 256) {
+            const uint32_t r = s.row(x);
+            dst[x] = reinterpret_cast<const T*>(s.at(r))[x - r * s.M];
+        }
+    } else {   // rows of more than 32 KB or so
+        for (uint64_t x = threadIdx.x; x < total; x += 256) {
+            const uint32_t r = (uint32_t)(x / s.M);
+            dst[x] = reinterpret_cast<const T*>(s.at(r))[x - (uint64_t)r * s.M];
+        }
+    }
+}
+
 __global__ void __launch_bounds__(256) gather_rows_multi_kernel(const RowsTable t, const int32_t* __restrict__ rows,
                                                                 int64_t K) {
-    int lo = 0, hi = t.n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (t.first[mid] <= blockIdx.x) lo = mid; else hi = mid - 1;
+    int k = 0, hi = t.n - 1;
+    while (k < hi) {
+        const int mid = (k + hi + 1) >> 1;
+        if (t.first[mid] <= blockIdx.x) k = mid; else hi = mid - 1;
     }
-    const uint32_t M = t.units[lo];
-    const int sh = t.unit_shift[lo];
-    const int64_t total = K * M;
-    const int64_t begin = (int64_t)(blockIdx.x - t.first[lo]) * ROWS_CHUNK;
-    const int64_t end = begin + ROWS_CHUNK < total ? begin + ROWS_CHUNK : total;
-    for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
-        const int64_t r = i / M;
-        const char* s = (const char*)t.src[lo] + (int64_t)rows[r] * t.pitch[lo] + ((i - r * M) << sh);
-        if (sh == 2) ((uint32_t*)t.dst[lo])[i] = *(const uint32_t*)s;
-        else if (sh == 1) ((uint16_t*)t.dst[lo])[i] = *(const uint16_t*)s;
-        else ((uint8_t*)t.dst[lo])[i] = *(const uint8_t*)s;
+    const uint32_t M = t.units[k];
+    const int sh = t.unit_shift[k];
+    const uint32_t R = rows_per_group(M, sh);
+    const int64_t row0 = (int64_t)(blockIdx.x - t.first[k]) * R;
+    const uint64_t count = (uint64_t)(K - row0 < (int64_t)R ? K - row0 : (int64_t)R);
+    const uint64_t total = count * M;
+    char* dst = (char*)t.dst[k] + ((row0 * M) << sh);
+    // x / M by one multiplication while x * M < 2^32, x < R * M
+    const uint32_t magic = M > 1 && (uint64_t)R * M * M < (1ull << 32) ? 0xffffffffu / M + 1 : 0;
+    const RowSource s = {(const char*)t.src[k], t.pitch[k], rows + row0, M, magic};
+    if (sh == 2 && ((uintptr_t)dst & 15) == 0 && (magic || M == 1)) {
+        // four units at a time: sixteen bytes of the copy, from one row or more
+        const uint32_t quads = (uint32_t)(total >> 2);
+        for (uint32_t q = threadIdx.x; q < quads; q += 256) {
+            uint32_t r = s.row(q << 2), c = (q << 2) - r * M, v[4];
+            const uint32_t* p = (const uint32_t*)s.at(r);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = p[c];
+                if (j < 3 && ++c == M) {
+                    c = 0;
+                    p = (const uint32_t*)s.at(++r);
+                }
+            }
+            reinterpret_cast<uint4*>(dst)[q] = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        const uint32_t x = (quads << 2) + threadIdx.x;
+        if (x < (uint32_t)total) {
+            const uint32_t r = s.row(x);
+            reinterpret_cast<uint32_t*>(dst)[x] = ((const uint32_t*)s.at(r))[x - r * M];
+        }
+    } else if (sh == 4) {
+        copy_units(s, (uint4*)dst, total);
+    } else if (sh == 3) {
+        copy_units(s, (uint2*)dst, total);
+    } else if (sh == 2) {
+        copy_units(s, (uint32_t*)dst, total);
+    } else if (sh == 1) {
+        copy_units(s, (uint16_t*)dst, total);
+    } else {
+        copy_units(s, (uint8_t*)dst, total);
     }
 }
 
@@ -221,6 +412,8 @@ __global__ void __launch_bounds__(256) gather_rows_multi_kernel(const RowsTable 
 hipError_t launch_accumulate_weights(int64_t N, float* weights, int views, const float* const* contributions,
                                      const float* opacity, float decay, hipStream_t st) {
     if (N <= 0) return hipSuccess;
+    uintptr_t bits = (uintptr_t)weights | (uintptr_t)opacity;
+    for (int v = 0; v < views; ++v) bits |= (uintptr_t)contributions[v];
     int first = 0;
     do {
         WeightArgs a;
@@ -230,15 +423,18 @@ hipError_t launch_accumulate_weights(int64_t N, float* weights, int views, const
         a.weights = weights;
         a.N = N;
         a.decay = first == 0 ? decay : 1.0f;
-        hipLaunchKernelGGL(accumulate_weights_kernel, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, st, a);
+        if ((bits & 15) == 0)
+            hipLaunchKernelGGL(accumulate_weights_kernel<4>, dim3((unsigned)((N + 1023) / 1024)), dim3(256), 0, st, a);
+        else
+            hipLaunchKernelGGL(accumulate_weights_kernel<1>, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, st, a);
         first += WEIGHT_VIEWS;
     } while (first < views);
     return hipGetLastError();
 }
 
 size_t evict_temp_bytes(int64_t N) {
-    const size_t nb = (size_t)((N + SELECT_ROWS - 1) / SELECT_ROWS);
-    return align_up(sizeof(SelectState), 256) + align_up((nb + 1) * sizeof(uint2), 256);
+    (void)N;
+    return align_up(sizeof(SelectState), 256) + SELECT_GROUPS * sizeof(uint2);
 }
 
 hipError_t launch_evict_select(int64_t N, const float* weights, int64_t budget, int64_t recent, int32_t* rows, void* temp,
@@ -253,14 +449,15 @@ hipError_t launch_evict_select(int64_t N, const float* weights, int64_t budget, 
     const int64_t old = N - recent;
     SelectState* s = (SelectState*)temp;
     uint2* counts = (uint2*)((char*)temp + align_up(sizeof(SelectState), 256));
-    const unsigned nb_old = (unsigned)((old + SELECT_ROWS - 1) / SELECT_ROWS), nb = (unsigned)((N + SELECT_ROWS - 1) / SELECT_ROWS);
+    const int64_t steps = (old + HIST_STEP - 1) / HIST_STEP, all = (N + SELECT_ROWS - 1) / SELECT_ROWS;
+    const int tiles = (int)((all + SELECT_GROUPS - 1) / SELECT_GROUPS);
+    const dim3 hist((unsigned)(steps < HIST_GROUPS ? steps : HIST_GROUPS)), groups((unsigned)((all + tiles - 1) / tiles));
     hipLaunchKernelGGL(select_clear_kernel, dim3(24), dim3(256), 0, st, s, (uint32_t)(keep - recent));
-    for (int pass = 0; pass < 3; ++pass) {
-        hipLaunchKernelGGL(select_hist_kernel, dim3(nb_old), dim3(SELECT_THREADS), 0, st, old, weights, s, pass);
-        hipLaunchKernelGGL(select_bin_kernel, dim3(1), dim3(256), 0, st, s, pass);
-    }
-    hipLaunchKernelGGL(select_count_kernel, dim3(nb), dim3(SELECT_THREADS), 0, st, N, old, weights, s, counts);
-    hipLaunchKernelGGL(select_write_kernel, dim3(nb), dim3(SELECT_THREADS), 0, st, N, old, weights, s, counts, rows);
+    hipLaunchKernelGGL(select_hist_kernel<0>, hist, dim3(HIST_THREADS), 0, st, old, weights, s);
+    hipLaunchKernelGGL(select_hist_kernel<1>, hist, dim3(HIST_THREADS), 0, st, old, weights, s);
+    hipLaunchKernelGGL(select_hist_kernel<2>, hist, dim3(HIST_THREADS), 0, st, old, weights, s);
+    hipLaunchKernelGGL(select_count_kernel, groups, dim3(SELECT_THREADS), 0, st, N, old, tiles, weights, s, counts);
+    hipLaunchKernelGGL(select_write_kernel, groups, dim3(SELECT_THREADS), 0, st, N, old, tiles, weights, s, counts, rows);
     return hipGetLastError();
 }
 
@@ -268,22 +465,23 @@ hipError_t launch_gather_rows_multi(int n, const GsoRowCopy* copies, const int32
     for (int i = 0; i < n;) {
         RowsTable t;
         t.n = 0;
-        t.first[0] = 0;
         int64_t chunks = 0;
         for (; i < n && t.n < ROWS_TABLE; ++i) {
             const GsoRowCopy& c = copies[i];
             if (c.row_bytes <= 0 || K <= 0) continue;
             const uint64_t bits = (uint64_t)c.row_bytes | (uint64_t)c.src_pitch | (uint64_t)(uintptr_t)c.src | (uint64_t)(uintptr_t)c.dst;
-            const int sh = (bits & 3) == 0 ? 2 : (bits & 1) == 0 ? 1 : 0;
-            const int64_t more = ((K * (c.row_bytes >> sh)) + ROWS_CHUNK - 1) / ROWS_CHUNK;
+            const int sh = (bits & 15) == 0 ? 4 : (bits & 7) == 0 ? 3 : (bits & 3) == 0 ? 2 : (bits & 1) == 0 ? 1 : 0;
+            const int64_t per = rows_per_group((uint32_t)(c.row_bytes >> sh), sh);
+            const int64_t more = (K + per - 1) / per;
             if (t.n > 0 && chunks + more > 0x7fffffff) break;
             t.src[t.n] = c.src;
             t.dst[t.n] = c.dst;
             t.pitch[t.n] = c.src_pitch;
             t.units[t.n] = (uint32_t)(c.row_bytes >> sh);
             t.unit_shift[t.n] = (uint8_t)sh;
+            t.first[t.n] = (uint32_t)chunks;
             chunks += more;
-            t.first[++t.n] = (uint32_t)chunks;
+            ++t.n;
         }
         if (t.n == 0) break;
         hipLaunchKernelGGL(gather_rows_multi_kernel, dim3((unsigned)chunks), dim3(256), 0, st, t, rows, K);

@@ -103,13 +103,14 @@ struct Norm {
     int partials = 0;
 };
 
-Norm sums_of(const Grads& g, int kind, void* st, const char* what) {
+Norm sums_of(const Grads& g, int kind, bool read_again, void* st, const char* what) {
     Norm r;
     const auto opt = torch::TensorOptions().device(g.own[0].device());
-    const size_t bytes = gso_norm_temp_bytes(g.n(), g.numel.data());
+    const size_t bytes = gso_norm_temp_bytes(g.n());
     r.temp = torch::empty({(int64_t)bytes}, opt.dtype(torch::kUInt8));
     r.value = torch::empty({}, opt.dtype(torch::kFloat32));
-    check_rc(gso_grad_norm(g.n(), g.cptr(), g.numel.data(), g.type.data(), kind, r.temp.data_ptr(), bytes, &r.partials, st),
+    check_rc(gso_grad_norm(g.n(), g.cptr(), g.numel.data(), g.type.data(), kind, read_again, r.temp.data_ptr(), bytes,
+                           &r.partials, st),
              what);
     return r;
 }
@@ -127,7 +128,7 @@ Tensor grad_norm(const std::vector<Tensor>& params, double norm_type) {
     if (g.own.empty()) return torch::zeros({});
     c10::DeviceGuard guard(g.own[0].device());
     void* st = stream_on(g.own[0].device());
-    Norm r = sums_of(g, kind, st, what);
+    Norm r = sums_of(g, kind, false, st, what);
     check_rc(gso_norm_finish(r.temp.data_ptr(), r.partials, kind, r.value.data_ptr<float>(), st), what);
     return r.value;
 }
@@ -142,7 +143,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& params, double max_norm, double
     c10::DeviceGuard guard(g.own[0].device());
     if (error_if_nonfinite) check_may_wait(what);
     void* st = stream_on(g.own[0].device());
-    Norm r = sums_of(g, kind, st, what);
+    Norm r = sums_of(g, kind, true, st, what);
     if (error_if_nonfinite) raise_if_nonfinite(r, kind, st, what);
     check_rc(gso_clip_grads(g.n(), g.ptr.data(), g.numel.data(), g.type.data(), kind, max_norm, r.temp.data_ptr(), r.partials,
                             r.value.data_ptr<float>(), st),
@@ -191,7 +192,7 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
         table.push_back(a);
     }
     void* st = stream_on(dev);
-    Norm r = sums_of(g, kind, st, what);
+    Norm r = sums_of(g, kind, false, st, what);
     if (error_if_nonfinite) raise_if_nonfinite(r, kind, st, what);
     check_rc(gso_adam_clipped((int)table.size(), table.data(), visible ? (const uint8_t*)visible->data_ptr() : nullptr, kind,
                               max_norm, r.temp.data_ptr(), r.partials, r.value.data_ptr<float>(), st),

@@ -456,8 +456,9 @@ int gso_gather_rows(const void* src, void* dst, const uint32_t* src_of_dst, int6
  *   c    = min(1, max_norm / (norm + 1e-6)), formed in 64 bits from the unrounded norm, rounded once to float32
  * `grads` are HOST arrays of n device pointers with their element counts and types (GsoType); elements are contiguous,
  * pointers aligned to an element, a count of zero (pointer ignored) is allowed.  Tensors may be of different types.
- *   gso_grad_norm: sums into `temp` (device, 8-byte aligned, gso_norm_temp_bytes(n, numels) bytes), *partials =
- *     how many sums it left there.
+ *   gso_grad_norm: sums into `temp` (device, 8-byte aligned, gso_norm_temp_bytes(n) bytes), *partials =
+ *     how many sums it left there.  read_again: nonzero when gso_clip_grads follows (the loads then leave what fits in
+ *     the caches).
  *   gso_norm_finish: *norm (device, float32) from `temp`.
  *   gso_clip_grads: the same, then g <- g * c in place, each product rounded once to the tensor's type; with c = 1
  *     nothing is read or written.  No two tensors may share memory.
@@ -475,9 +476,9 @@ typedef struct {
     int64_t width;
     double lr, beta1, beta2, eps, bias_correction1, bias_correction2_sqrt;   /* as gso_adam_update takes them */
 } GsoAdamTensor;
-size_t gso_norm_temp_bytes(int n, const int64_t* numels);
-int gso_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type, void* temp,
-                  size_t temp_bytes, int* partials, void* stream);
+size_t gso_norm_temp_bytes(int n);
+int gso_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type, int read_again,
+                  void* temp, size_t temp_bytes, int* partials, void* stream);
 int gso_norm_finish(void* temp, int partials, int norm_type, float* norm, void* stream);
 int gso_clip_grads(int n, void* const* grads, const int64_t* numels, const int* types, int norm_type, double max_norm,
                    void* temp, int partials, float* norm, void* stream);

@@ -69,11 +69,11 @@ def test_c_abi_refuses_bad_arguments():
     t0, t9 = (C.c_int * 1)(0), (C.c_int * 1)(9)
     good, odd, null = (C.c_void_p * 1)(4096), (C.c_void_p * 1)(4097), (C.c_void_p * 1)(None)
     cnt = C.c_int(0)
-    size = L.gso_norm_temp_bytes(1, one)
-    assert size > 0 and L.gso_norm_temp_bytes(-1, one) == 0 and L.gso_norm_temp_bytes(0, None) > 0
+    size = L.gso_norm_temp_bytes(1)
+    assert size > 0 and L.gso_norm_temp_bytes(-1) == 0 and L.gso_norm_temp_bytes(0) > 0
 
     def norm(n=1, g=good, k=one, t=t0, kind=2, temp=4096, bytes_=size, out=C.byref(cnt)):
-        return L.gso_grad_norm(n, g, k, t, kind, temp, bytes_, out, None)
+        return L.gso_grad_norm(n, g, k, t, kind, 0, temp, bytes_, out, None)
     assert norm(n=-1) == ARG and norm(g=null) == ARG and norm(g=odd) == ARG and norm(k=neg) == ARG and norm(t=t9) == ARG
     assert norm(kind=3) == ARG and norm(kind=-1) == ARG and norm(temp=None) == ARG and norm(temp=4100) == ARG
     assert norm(out=None) == ARG and norm(g=None) == ARG and norm(bytes_=8) == BUFFER
