@@ -331,30 +331,106 @@ __host__ __device__ inline uint32_t rows_per_group(uint32_t units, int unit_shif
     return r < 16 ? 16u : r & ~15u;
 }
 
-// Where unit x of a run of rows lies in the source.
-struct RowSource {
+// A run of rows: unit x of the copy is unit x mod M of row rows[x / M].
+struct RowRun {
     const char* src;
     int64_t pitch;
     const int32_t* rows;
     uint32_t M, magic;
-    // x < 2^32, and M = 1 or a multiplier for M
+    // x / M for x < 2^32, by one multiplication where x * M < 2^32 (magic = 0: it is not, or M = 1)
     __device__ __forceinline__ uint32_t row(uint32_t x) const { return M == 1 ? x : (uint32_t)(((uint64_t)x * magic) >> 32); }
     __device__ __forceinline__ const char* at(uint32_t r) const { return src + (int64_t)rows[r] * pitch; }
 };
 
+// Unit by unit: rows of more than about 32 KB, whose units a multiplication cannot divide, and copies that do not start
+// at a multiple of sixteen bytes.
 template <typename T>
-__device__ __forceinline__ void copy_units(const RowSource& s, T* __restrict__ dst, uint64_t total) {
-    if (s.magic || s.M == 1) {
-        for (uint32_t x = threadIdx.x; x < (uint32_t)total; x += 256) {
-            const uint32_t r = s.row(x);
-            dst[x] = reinterpret_cast<const T*>(s.at(r))[x - r * s.M];
-        }
-    } else {   // rows of more than 32 KB or so
-        for (uint64_t x = threadIdx.x; x < total; x += 256) {
-            const uint32_t r = (uint32_t)(x / s.M);
-            dst[x] = reinterpret_cast<const T*>(s.at(r))[x - (uint64_t)r * s.M];
-        }
+__device__ __forceinline__ void copy_units(const RowRun& s, T* __restrict__ dst, uint64_t total) {
+    for (uint64_t x = threadIdx.x; x < total; x += 256) {
+        const uint32_t r = (uint32_t)(x / s.M);
+        dst[x] = reinterpret_cast<const T*>(s.at(r))[x - (uint64_t)r * s.M];
     }
+}
+
+// Sixteen bytes of the copy at a time.  They lie side by side in the source as well when they are in one row, or in rows
+// that follow each other there: then one load fetches them, which needs no alignment of its own.
+template <typename T>
+using vector_of = f32x4 __attribute__((aligned(sizeof(T))));
+
+// At most two rows in a vector.  Four vectors are in flight per thread, and all row numbers are read before the first of
+// them: loads return in order, and a row number behind a vector would wait for it.
+template <typename T>
+__device__ __forceinline__ void copy_wide(const RowRun& s, T* __restrict__ dst, uint32_t vectors) {
+    constexpr uint32_t N = 16 / sizeof(T);
+    for (uint32_t q0 = threadIdx.x; q0 < vectors; q0 += 4 * 256) {
+        const T *here[4], *next[4];   // unit j of a vector is here[j], or next[j] behind the row's end
+        uint32_t left[4];             // units of the vector's first row
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t x = (q0 + u * 256 < vectors ? q0 + u * 256 : q0) * N, r = s.row(x), c = x - r * s.M;
+            here[u] = next[u] = reinterpret_cast<const T*>(s.at(r)) + c;
+            left[u] = s.M - c;
+            if (left[u] < N) next[u] = reinterpret_cast<const T*>(s.at(r + 1)) - left[u];
+        }
+        f32x4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (here[u] == next[u]) {
+                v[u] = *reinterpret_cast<const vector_of<T>*>(here[u]);
+            } else {
+                union { f32x4 v; T t[N]; } e;
+#pragma unroll
+                for (uint32_t j = 0; j < N; ++j) e.t[j] = (j < left[u] ? here[u] : next[u])[j];
+                v[u] = e.v;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (q0 + u * 256 < vectors) __builtin_nontemporal_store(v[u], (f32x4*)dst + q0 + u * 256);
+    }
+}
+
+// Three rows and more in a vector.
+template <typename T>
+__device__ __forceinline__ void copy_narrow(const RowRun& s, T* __restrict__ dst, uint32_t vectors) {
+    constexpr uint32_t N = 16 / sizeof(T);
+    const bool dense = s.pitch == (int64_t)(s.M * sizeof(T));
+    for (uint32_t q = threadIdx.x; q < vectors; q += 256) {
+        const uint32_t x = q * N, r0 = s.row(x), c0 = x - r0 * s.M;
+        int32_t at[N];
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) at[j] = s.rows[s.row(x + j)];
+        f32x4 v;
+        if (dense && at[N - 1] - at[0] == (int32_t)(s.row(x + N - 1) - r0)) {   // rows ascend
+            v = *reinterpret_cast<const vector_of<T>*>(s.src + (int64_t)at[0] * s.pitch + c0 * sizeof(T));
+        } else {
+            union { f32x4 v; T t[N]; } e;
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j)
+                e.t[j] = reinterpret_cast<const T*>(s.src + (int64_t)at[j] * s.pitch)[x + j - s.row(x + j) * s.M];
+            v = e.v;
+        }
+        __builtin_nontemporal_store(v, (f32x4*)dst + q);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void copy_run(const RowRun& s, T* __restrict__ dst, uint32_t total) {
+    constexpr uint32_t N = 16 / sizeof(T);
+    const uint32_t vectors = total / N;
+    if (s.M + 1 >= N) copy_wide<T>(s, dst, vectors);
+    else copy_narrow<T>(s, dst, vectors);
+    const uint32_t x = vectors * N + threadIdx.x;
+    if (x < total) {
+        const uint32_t r = s.row(x);
+        dst[x] = reinterpret_cast<const T*>(s.at(r))[x - r * s.M];
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void copy_rows(const RowRun& s, char* dst, uint64_t total) {
+    if ((s.magic || s.M == 1) && ((uintptr_t)dst & 15) == 0) copy_run<T>(s, (T*)dst, (uint32_t)total);
+    else copy_units<T>(s, (T*)dst, total);
 }
 
 __global__ void __launch_bounds__(256) gather_rows_multi_kernel(const RowsTable t, const int32_t* __restrict__ rows,
@@ -368,44 +444,15 @@ __global__ void __launch_bounds__(256) gather_rows_multi_kernel(const RowsTable 
     const int sh = t.unit_shift[k];
     const uint32_t R = rows_per_group(M, sh);
     const int64_t row0 = (int64_t)(blockIdx.x - t.first[k]) * R;
-    const uint64_t count = (uint64_t)(K - row0 < (int64_t)R ? K - row0 : (int64_t)R);
-    const uint64_t total = count * M;
+    const uint64_t total = (uint64_t)(K - row0 < (int64_t)R ? K - row0 : (int64_t)R) * M;
     char* dst = (char*)t.dst[k] + ((row0 * M) << sh);
-    // x / M by one multiplication while x * M < 2^32, x < R * M
     const uint32_t magic = M > 1 && (uint64_t)R * M * M < (1ull << 32) ? 0xffffffffu / M + 1 : 0;
-    const RowSource s = {(const char*)t.src[k], t.pitch[k], rows + row0, M, magic};
-    if (sh == 2 && ((uintptr_t)dst & 15) == 0 && (magic || M == 1)) {
-        // four units at a time: sixteen bytes of the copy, from one row or more
-        const uint32_t quads = (uint32_t)(total >> 2);
-        for (uint32_t q = threadIdx.x; q < quads; q += 256) {
-            uint32_t r = s.row(q << 2), c = (q << 2) - r * M, v[4];
-            const uint32_t* p = (const uint32_t*)s.at(r);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = p[c];
-                if (j < 3 && ++c == M) {
-                    c = 0;
-                    p = (const uint32_t*)s.at(++r);
-                }
-            }
-            reinterpret_cast<uint4*>(dst)[q] = make_uint4(v[0], v[1], v[2], v[3]);
-        }
-        const uint32_t x = (quads << 2) + threadIdx.x;
-        if (x < (uint32_t)total) {
-            const uint32_t r = s.row(x);
-            reinterpret_cast<uint32_t*>(dst)[x] = ((const uint32_t*)s.at(r))[x - r * M];
-        }
-    } else if (sh == 4) {
-        copy_units(s, (uint4*)dst, total);
-    } else if (sh == 3) {
-        copy_units(s, (uint2*)dst, total);
-    } else if (sh == 2) {
-        copy_units(s, (uint32_t*)dst, total);
-    } else if (sh == 1) {
-        copy_units(s, (uint16_t*)dst, total);
-    } else {
-        copy_units(s, (uint8_t*)dst, total);
-    }
+    const RowRun s = {(const char*)t.src[k], t.pitch[k], rows + row0, M, magic};
+    if (sh == 4) copy_rows<f32x4>(s, dst, total);
+    else if (sh == 3) copy_rows<uint2>(s, dst, total);
+    else if (sh == 2) copy_rows<uint32_t>(s, dst, total);
+    else if (sh == 1) copy_rows<uint16_t>(s, dst, total);
+    else copy_rows<uint8_t>(s, dst, total);
 }
 
 // ------------------------------------------------------------------ host
