@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(256) accumulate_weights_kernel(const WeightArg
 constexpr int HIST_BINS = 2048;
 constexpr int HIST_THREADS = 1024;
 constexpr int HIST_GROUPS = 512;        // two workgroups per CU: each adds its whole histogram to the global one once
-constexpr int HIST_STEP = 4 * HIST_THREADS;
+constexpr int HIST_STEP = 16 * HIST_THREADS;
 constexpr int SELECT_THREADS = 256;
 constexpr int SELECT_ROWS = 4096;       // rows of a tile: sixteen a thread
 constexpr int SELECT_GROUPS = 2048;     // workgroups of the counting and writing kernels, a run of tiles each
@@ -163,22 +163,26 @@ __global__ void __launch_bounds__(HIST_THREADS) select_hist_kernel(int64_t old, 
     }
     const bool aligned = ((uintptr_t)weights & 15) == 0;
     for (int64_t base = (int64_t)blockIdx.x * HIST_STEP; base < old; base += (int64_t)gridDim.x * HIST_STEP) {
-        const int64_t i = base + 4 * (int)threadIdx.x;
-        float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (aligned && i + 4 <= old) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(weights + i);
+        f32x4 w[4];   // sixteen keys a thread in flight
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = x[j];
-        } else {
+        for (int q = 0; q < 4; ++q) {
+            const int64_t i = base + 4 * (q * HIST_THREADS + (int)threadIdx.x);
+            if (aligned && i + 4 <= old) {
+                w[q] = *reinterpret_cast<const f32x4*>(weights + i);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (i + j < old) w[j] = weights[i + j];
+                for (int j = 0; j < 4; ++j) w[q][j] = i + j < old ? weights[i + j] : 0.0f;
+            }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t k = weight_key(w[j]);
-            const bool in = i + j < old && (PASS == 0 || (uint32_t)((uint64_t)k >> (shift + bits)) == prefix);
-            hist_add(h, (k >> shift) & ((1u << bits) - 1), in);
+        for (int q = 0; q < 4; ++q) {
+            const int64_t i = base + 4 * (q * HIST_THREADS + (int)threadIdx.x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t k = weight_key(w[q][j]);
+                const bool in = i + j < old && (PASS == 0 || (uint32_t)((uint64_t)k >> (shift + bits)) == prefix);
+                hist_add(h, (k >> shift) & ((1u << bits) - 1), in);
+            }
         }
     }
     __syncthreads();

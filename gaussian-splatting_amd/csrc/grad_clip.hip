@@ -20,7 +20,8 @@ constexpr int NORM_TABLE = 240;     // tensors per launch of the norm and scale 
 constexpr int NORM_GROUPS = 2048;   // workgroups of the norm kernel: eight per CU
 constexpr int ADAM_TABLE = 40;      // tensors per launch of the Adam kernel
 constexpr int CHUNK_BYTES = 16384;  // a chunk of a tensor, from its start rounded down to 16 bytes: four vectors a thread
-constexpr int ADAM_CHUNK = 2048;    // elements of a chunk of the Adam kernel: two vectors a thread
+constexpr int ADAM_CHUNK = 2048;    // elements of a workgroup of the dense Adam kernel: two vectors a thread
+constexpr int SPARSE_CHUNK = 8192;  // elements of the rows of a workgroup of the sparse one, about
 
 // 16 bytes per tensor.
 struct NormTable {
@@ -36,13 +37,13 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 struct AdamEntry {
     float *param, *exp_avg, *exp_avg_sq;
     const float* grad;
-    int64_t numel;
-    uint32_t width;                   // elements per row, for the visibility flags
+    int64_t count;                    // elements, or rows for the sparse kernel
+    uint32_t width;                   // elements per row
     AdamConst c;
 };
 struct AdamTable {
     AdamEntry e[ADAM_TABLE];
-    uint32_t first[ADAM_TABLE + 1];
+    uint32_t first[ADAM_TABLE];       // first workgroup of each tensor
     int n;
 };
 
@@ -276,64 +277,23 @@ __global__ void __launch_bounds__(NORM_THREADS) scale_kernel(const NormTable t, 
     });
 }
 
-// x / d for x * d < 2^32 by one multiplication (magic = floor(2^32 / d) + 1: too large by less than d / 2^32 of x),
-// by a division for wider rows.
-struct RowDivider {
-    uint32_t width, magic;
-    __device__ __forceinline__ explicit RowDivider(uint32_t w) : width(w), magic(w > 1 && w <= 32768 ? 0xffffffffu / w + 1 : 0) {}
-    __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
-        return magic ? (uint32_t)(((uint64_t)x * magic) >> 32) : width == 1 ? x : x / width;
-    }
-};
-
 // Two vectors of each stream a thread, all loads first, non-temporal: every value is used once in a step.
-template <bool SPARSE>
-__global__ void __launch_bounds__(NORM_THREADS) adam_clipped_kernel(const AdamTable t, const uint8_t* __restrict__ visible,
-                                                                    const NormResult* __restrict__ result) {
+__global__ void __launch_bounds__(NORM_THREADS) adam_clipped_kernel(const AdamTable t, const NormResult* __restrict__ result) {
     const float s = result->coefficient;
-    int k = 0;
-    {
-        int hi = t.n - 1;
-        while (k < hi) {
-            const int mid = (k + hi + 1) >> 1;
-            if (t.first[mid] <= blockIdx.x) k = mid; else hi = mid - 1;
-        }
-    }
+    const int k = find_tensor(t, blockIdx.x);
     const AdamEntry& e = t.e[k];
     const int64_t base = (int64_t)(blockIdx.x - t.first[k]) * ADAM_CHUNK;
-    const int count = e.numel - base < ADAM_CHUNK ? (int)(e.numel - base) : ADAM_CHUNK;
+    const int count = e.count - base < ADAM_CHUNK ? (int)(e.count - base) : ADAM_CHUNK;
     float *p = e.param + base, *m = e.exp_avg + base, *v = e.exp_avg_sq + base;
     const float* g = e.grad + base;
-    const uint32_t W = e.width;
-    int64_t row0 = 0;
-    uint32_t rem0 = 0;
-    if (SPARSE) {
-        row0 = base / W;
-        rem0 = (uint32_t)(base - row0 * W);
-    }
-    const RowDivider rows(W);
-    const uint8_t* seen = SPARSE ? visible + row0 : nullptr;
-    if (((((uintptr_t)p | (uintptr_t)m | (uintptr_t)v | (uintptr_t)g) & 15) == 0)) {
+    int done = 0;
+    if ((((uintptr_t)p | (uintptr_t)m | (uintptr_t)v | (uintptr_t)g) & 15) == 0) {
+        done = count & ~3;
         f32x4 P[2], G[2], M[2], V[2];
-        uint32_t on[2];   // one bit per element
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int i = 4 * (u * NORM_THREADS + (int)threadIdx.x);
-            on[u] = i + 4 <= count ? 15u : 0u;
-            if (SPARSE && on[u]) {
-                const uint32_t x = rem0 + (uint32_t)i;
-                uint32_t r = rows(x), rem = x - r * W;
-                on[u] = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (seen[r]) on[u] |= 1u << j;
-                    if (++rem == W) {
-                        rem = 0;
-                        ++r;
-                    }
-                }
-            }
-            if (on[u]) {
+            if (i < done) {
                 P[u] = __builtin_nontemporal_load((const f32x4*)(p + i));
                 G[u] = __builtin_nontemporal_load((const f32x4*)(g + i));
                 M[u] = __builtin_nontemporal_load((const f32x4*)(m + i));
@@ -343,35 +303,90 @@ __global__ void __launch_bounds__(NORM_THREADS) adam_clipped_kernel(const AdamTa
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int i = 4 * (u * NORM_THREADS + (int)threadIdx.x);
-            if (!on[u]) continue;
+            if (i < done) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float mm = M[u][j], vv = V[u][j];
-                const float pp = adam_update(P[u][j], G[u][j] * s, &mm, &vv, e.c);
-                if (!SPARSE || (on[u] >> j & 1u)) {   // a vector belongs to one thread: its other elements are stored as they were
-                    P[u][j] = pp;
+                for (int j = 0; j < 4; ++j) {
+                    float mm = M[u][j], vv = V[u][j];
+                    P[u][j] = adam_update(P[u][j], G[u][j] * s, &mm, &vv, e.c);
                     M[u][j] = mm;
                     V[u][j] = vv;
                 }
+                __builtin_nontemporal_store(P[u], (f32x4*)(p + i));
+                __builtin_nontemporal_store(M[u], (f32x4*)(m + i));
+                __builtin_nontemporal_store(V[u], (f32x4*)(v + i));
             }
-            __builtin_nontemporal_store(P[u], (f32x4*)(p + i));
-            __builtin_nontemporal_store(M[u], (f32x4*)(m + i));
-            __builtin_nontemporal_store(V[u], (f32x4*)(v + i));
         }
-        const int i = (count & ~3) + (int)threadIdx.x;   // the last elements of the tensor
-        if (i < count && (!SPARSE || seen[rows(rem0 + (uint32_t)i)])) {
-            float mm = m[i], vv = v[i];
-            p[i] = adam_update(p[i], g[i] * s, &mm, &vv, e.c);
-            m[i] = mm;
-            v[i] = vv;
+    }
+    for (int i = done + (int)threadIdx.x; i < count; i += NORM_THREADS) {
+        float mm = m[i], vv = v[i];
+        p[i] = adam_update(p[i], g[i] * s, &mm, &vv, e.c);
+        m[i] = mm;
+        v[i] = vv;
+    }
+}
+
+// The sparse step touches few rows (a view sees about a tenth of a large scene), so a thread per element of all rows
+// would leave most lanes without a load: the workgroup first lists its visible rows, then its threads walk the elements
+// of the listed rows only, four each in flight.  The list's order is that of arrival; every element is updated on
+// its own, so nothing depends on it.
+__global__ void __launch_bounds__(NORM_THREADS) adam_clipped_sparse_kernel(const AdamTable t, const uint8_t* __restrict__ visible,
+                                                                           const NormResult* __restrict__ result) {
+    __shared__ uint16_t s_row[SPARSE_CHUNK];
+    __shared__ uint32_t s_count;
+    const float s = result->coefficient;
+    const int k = find_tensor(t, blockIdx.x);
+    const AdamEntry& e = t.e[k];
+    const uint32_t W = e.width, R = W < SPARSE_CHUNK ? SPARSE_CHUNK / W : 1;
+    const int64_t row0 = (int64_t)(blockIdx.x - t.first[k]) * R;
+    const uint32_t nrows = e.count - row0 < (int64_t)R ? (uint32_t)(e.count - row0) : R;
+    if (threadIdx.x == 0) s_count = 0;
+    __syncthreads();
+    const int lane = threadIdx.x & (WAVE - 1);
+    for (uint32_t r0 = 0; r0 < nrows; r0 += 4 * NORM_THREADS) {
+        bool on[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t r = r0 + u * NORM_THREADS + threadIdx.x;
+            on[u] = r < nrows && visible[row0 + r] != 0;
         }
-    } else {
-        for (int i = threadIdx.x; i < count; i += NORM_THREADS) {
-            if (SPARSE && !seen[rows(rem0 + (uint32_t)i)]) continue;
-            float mm = m[i], vv = v[i];
-            p[i] = adam_update(p[i], g[i] * s, &mm, &vv, e.c);
-            m[i] = mm;
-            v[i] = vv;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint64_t mask = __ballot(on[u]);
+            if (mask == 0) continue;
+            uint32_t at = 0;
+            if (lane == 0) at = atomicAdd(&s_count, (uint32_t)__popcll(mask));
+            at = (uint32_t)__builtin_amdgcn_readlane((int)at, 0) + (uint32_t)__popcll(mask & ((1ull << lane) - 1));
+            if (on[u]) s_row[at] = (uint16_t)(r0 + u * NORM_THREADS + threadIdx.x);
+        }
+    }
+    __syncthreads();
+    const uint32_t total = s_count * W;   // less than SPARSE_CHUNK, or one row
+    // x / W by one multiplication: x and W stay below 2^13 unless the row is the only one
+    const uint32_t magic = W > 1 && W < SPARSE_CHUNK ? 0xffffffffu / W + 1 : 0;
+    float *p = e.param + row0 * W, *m = e.exp_avg + row0 * W, *v = e.exp_avg_sq + row0 * W;
+    const float* g = e.grad + row0 * W;
+    for (uint32_t x0 = threadIdx.x; x0 < total; x0 += 4 * NORM_THREADS) {
+        uint32_t i[4];
+        float P[4], G[4], M[4], V[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t x = x0 + u * NORM_THREADS < total ? x0 + u * NORM_THREADS : x0;
+            const uint32_t n = W == 1 ? x : (uint32_t)(((uint64_t)x * magic) >> 32);
+            i[u] = (uint32_t)s_row[n] * W + (x - n * W);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            P[u] = p[i[u]];
+            G[u] = g[i[u]];
+            M[u] = m[i[u]];
+            V[u] = v[i[u]];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (x0 + u * NORM_THREADS >= total) break;
+            p[i[u]] = adam_update(P[u], G[u] * s, &M[u], &V[u], e.c);
+            m[i[u]] = M[u];
+            v[i[u]] = V[u];
         }
     }
 }
@@ -470,20 +485,23 @@ hipError_t launch_adam_clipped(int n, const GsoAdamTensor* tensors, const uint8_
     for (int i = 0; i < n && e == hipSuccess;) {
         AdamTable t;
         t.n = 0;
-        t.first[0] = 0;
+        int64_t groups = 0;
         for (; i < n && t.n < ADAM_TABLE; ++i) {
             const GsoAdamTensor& a = tensors[i];
-            const int64_t numel = a.rows * a.width;
+            const int64_t numel = a.rows * a.width, R = a.width < SPARSE_CHUNK ? SPARSE_CHUNK / a.width : 1;
             if (numel <= 0) continue;
-            t.e[t.n] = {a.param, a.exp_avg, a.exp_avg_sq, a.grad, numel, (uint32_t)a.width,
+            const int64_t more = visible ? (a.rows + R - 1) / R : (numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
+            if (t.n > 0 && groups + more > 0x7fffffff) break;
+            t.e[t.n] = {a.param, a.exp_avg, a.exp_avg_sq, a.grad, visible ? a.rows : numel, (uint32_t)a.width,
                         adam_const(a.lr, a.beta1, a.beta2, a.eps, a.bias_correction1, a.bias_correction2_sqrt)};
-            t.first[t.n + 1] = t.first[t.n] + (uint32_t)((numel + ADAM_CHUNK - 1) / ADAM_CHUNK);
+            t.first[t.n] = (uint32_t)groups;
+            groups += more;
             ++t.n;
         }
         if (t.n == 0) break;
-        const dim3 grid(t.first[t.n]), block(NORM_THREADS);
-        if (visible) hipLaunchKernelGGL(adam_clipped_kernel<true>, grid, block, 0, st, t, visible, (const NormResult*)temp);
-        else hipLaunchKernelGGL(adam_clipped_kernel<false>, grid, block, 0, st, t, visible, (const NormResult*)temp);
+        const dim3 grid((unsigned)groups), block(NORM_THREADS);
+        if (visible) hipLaunchKernelGGL(adam_clipped_sparse_kernel, grid, block, 0, st, t, visible, (const NormResult*)temp);
+        else hipLaunchKernelGGL(adam_clipped_kernel, grid, block, 0, st, t, (const NormResult*)temp);
         e = hipGetLastError();
     }
     return e;

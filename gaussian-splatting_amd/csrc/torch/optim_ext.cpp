@@ -49,6 +49,7 @@ struct Grads {
 };
 
 Grads collect(const std::vector<Tensor>& params, const char* what) {
+    torch::NoGradGuard no_grad;
     Grads g;
     const size_t n = params.size();
     g.own.reserve(n);
@@ -148,6 +149,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& params, double max_norm, double
     check_rc(gso_clip_grads(g.n(), g.ptr.data(), g.numel.data(), g.type.data(), kind, max_norm, r.temp.data_ptr(), r.partials,
                             r.value.data_ptr<float>(), st),
              what);
+    torch::NoGradGuard no_grad;
     for (size_t i = 0; i < g.own.size(); ++i)
         if (!g.packed[i].is_same(g.own[i])) g.own[i].copy_(g.packed[i]);
     return r.value;
@@ -203,6 +205,7 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
 void accumulate_weights(const Tensor& weights, const std::vector<Tensor>& contributions, const c10::optional<Tensor>& opacity,
                         double decay) {
     const char* what = "accumulate_weights";
+    torch::NoGradGuard no_grad;
     const int64_t N = weights.numel();
     std::vector<const float*> ptr;
     std::vector<Tensor> keep;
@@ -229,6 +232,7 @@ void accumulate_weights(const Tensor& weights, const std::vector<Tensor>& contri
 }
 
 Tensor evict_select(const Tensor& weights, int64_t budget, int64_t recent) {
+    torch::NoGradGuard no_grad;
     const char* what = "evict_rows";
     TORCH_CHECK(weights.is_cuda(), what, ": weights must be a GPU tensor (there is no CPU path)");
     const int64_t N = weights.numel();
@@ -251,6 +255,7 @@ Tensor evict_select(const Tensor& weights, int64_t budget, int64_t recent) {
 std::vector<Tensor> take_rows(const std::vector<Tensor>& tensors, const Tensor& rows, int64_t N) {
     const char* what = "evict_rows";
     const int64_t K = rows.numel();
+    torch::NoGradGuard no_grad;
     std::vector<Tensor> out, keep;
     std::vector<GsoRowCopy> copies;
     out.reserve(tensors.size());
@@ -258,7 +263,7 @@ std::vector<Tensor> take_rows(const std::vector<Tensor>& tensors, const Tensor& 
         TORCH_CHECK(t.layout() == c10::kStrided && t.device() == rows.device() && t.dim() >= 1 && t.size(0) == N, what,
                     ": every tensor needs one row per weight (", N, ") on ", rows.device(), ", got ", t.sizes(), " on ", t.device());
         // rows that are packed in themselves may lie any distance apart; others are packed first
-        const Tensor s = (K > 0 && t.numel() > 0 && t.select(0, 0).is_contiguous()) ? t : t.contiguous();
+        const Tensor s = t.is_contiguous() || (N > 0 && t.numel() > 0 && t.select(0, 0).is_contiguous()) ? t : t.contiguous();
         std::vector<int64_t> shape = s.sizes().vec();
         shape[0] = K;
         out.push_back(torch::empty(shape, s.options()));

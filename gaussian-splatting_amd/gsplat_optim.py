@@ -83,20 +83,25 @@ class FusedGaussianAdam(torch.optim.Adam):
 
 
 # ---------------------------------------------------------------- gradient norm and clipping
+_host_layer = None
+
+
 def _host():
     """The compiled host layer (csrc/torch/optim_ext.cpp)."""
-    from diff_gaussian_rasterization import _C
-    if _C._hip_ext is None:
-        raise ImportError("the PyTorch host extension is missing or was replaced by a library override: build it with "
-                          "`python gaussian-splatting_amd/csrc/torch/build_ext.py` (there is no CPU fallback)")
-    return _C._hip_ext
+    global _host_layer
+    if _host_layer is None:
+        from diff_gaussian_rasterization import _C
+        if _C._hip_ext is None:
+            raise ImportError("the PyTorch host extension is missing or was replaced by a library override: build it with "
+                              "`python gaussian-splatting_amd/csrc/torch/build_ext.py` (there is no CPU fallback)")
+        _host_layer = _C._hip_ext
+    return _host_layer
 
 
 def _tensors(parameters):
     return [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
 
 
-@torch.no_grad()
 def grad_norm(parameters, norm_type=2.0):
     """The norm of all the gradients of `parameters` (an iterable of tensors, or one) together, as if they were one
     vector: norm_type 2, 1 or inf.  A 0-d float32 tensor on the gradients' device; the host does not wait for it.
@@ -108,7 +113,6 @@ def grad_norm(parameters, norm_type=2.0):
     return _host().grad_norm(_tensors(parameters), float(norm_type))
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_: scales the gradients in place by min(1, max_norm / (norm + 1e-6)) and returns
     the norm they had (`grad_norm`).  Under the ceiling the gradients are read once and not written.  As there, a
@@ -435,7 +439,6 @@ def densify_and_prune(optimizer, stats, max_grad, min_opacity, extent, max_scree
 
 
 # ---------------------------------------------------------------- a model within a row budget
-@torch.no_grad()
 def accumulate_weights(weights, contributions, opacity=None, decay=1.0):
     """Adds what some views say about how much each Gaussian matters, in place and in one pass:
 
@@ -451,7 +454,6 @@ def accumulate_weights(weights, contributions, opacity=None, decay=1.0):
     return weights
 
 
-@torch.no_grad()
 def evict_rows(weights, budget, recent=0, tensors=()):
     """Which rows stay when a model of N rows may have only `budget`, and those rows of `tensors`.
 
