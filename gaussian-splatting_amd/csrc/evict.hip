@@ -70,7 +70,6 @@ __global__ void __launch_bounds__(256) accumulate_weights_kernel(const WeightArg
 constexpr int HIST_BINS = 2048;
 constexpr int HIST_THREADS = 1024;
 constexpr int HIST_GROUPS = 512;        // two workgroups per CU: each adds its whole histogram to the global one once
-constexpr int HIST_STEP = 16 * HIST_THREADS;
 constexpr int SELECT_THREADS = 256;
 constexpr int SELECT_ROWS = 4096;       // rows of a tile: sixteen a thread
 constexpr int SELECT_GROUPS = 2048;     // workgroups of the counting and writing kernels, a run of tiles each
@@ -134,25 +133,17 @@ __device__ __forceinline__ uint2 find_bin(const SelectState* __restrict__ s) {
     return s_found;
 }
 
-// Adds one to a bin for each lane that is `in`.  Weights repeat (rows that no view has seen are all zero): the lanes
-// that share the first active lane's bin are counted with one ballot and added at once, the others one by one.
-__device__ __forceinline__ void hist_add(uint32_t* h, uint32_t bin, bool in) {
-    const uint64_t act = __ballot(in);
-    if (act == 0) return;
-    const int leader = __builtin_ctzll(act);
-    const uint32_t common = (uint32_t)__builtin_amdgcn_readlane((int)bin, leader);
-    const bool same = in && bin == common;
-    const uint64_t m = __ballot(same);
-    if ((int)(threadIdx.x & 63) == leader) atomicAdd(&h[common], (uint32_t)__popcll(m));
-    else if (in && !same) atomicAdd(&h[bin], 1u);
-}
+constexpr int HIST_COPIES = 4;   // of the workgroup's histogram, side by side: few bins hold most weights
 
-template <int PASS>
+// VECS: 16-byte loads a thread has in flight.  The rows that no view has seen all weigh zero; they are counted per wave
+// with a ballot, and only the others go to LDS.
+template <int PASS, int VECS>
 __global__ void __launch_bounds__(HIST_THREADS) select_hist_kernel(int64_t old, const float* __restrict__ weights,
                                                                    SelectState* __restrict__ s) {
-    __shared__ uint32_t h[HIST_BINS];
-    constexpr int shift = pass_shift(PASS), bits = pass_bits(PASS);
-    for (int b = threadIdx.x; b < HIST_BINS; b += HIST_THREADS) h[b] = 0;
+    __shared__ uint32_t h[HIST_BINS * HIST_COPIES];
+    constexpr int shift = pass_shift(PASS), bits = pass_bits(PASS), step = 4 * VECS * HIST_THREADS;
+    constexpr uint32_t ZERO = 0x80000000u;   // weight_key(0)
+    for (int b = threadIdx.x; b < HIST_BINS * HIST_COPIES; b += HIST_THREADS) h[b] = 0;
     uint32_t prefix = 0;
     if (PASS > 0) {
         const uint2 at = find_bin<(PASS > 0 ? PASS - 1 : 0), HIST_THREADS>(s);
@@ -161,33 +152,43 @@ __global__ void __launch_bounds__(HIST_THREADS) select_hist_kernel(int64_t old, 
     } else {
         __syncthreads();
     }
+    uint32_t* own = h + (threadIdx.x & (HIST_COPIES - 1));
+    const bool count_zeros = PASS == 0 || (uint32_t)((uint64_t)ZERO >> (shift + bits)) == prefix;
+    uint32_t zeros = 0;
+    auto add = [&](float w, bool valid) {
+        const uint32_t k = weight_key(w);
+        zeros += (uint32_t)__popcll(__ballot(valid && k == ZERO));
+        const bool in = valid && k != ZERO && (PASS == 0 || (uint32_t)((uint64_t)k >> (shift + bits)) == prefix);
+        if (in) atomicAdd(own + ((k >> shift) & ((1u << bits) - 1)) * HIST_COPIES, 1u);
+    };
     const bool aligned = ((uintptr_t)weights & 15) == 0;
-    for (int64_t base = (int64_t)blockIdx.x * HIST_STEP; base < old; base += (int64_t)gridDim.x * HIST_STEP) {
-        f32x4 w[4];   // sixteen keys a thread in flight
+    for (int64_t base = (int64_t)blockIdx.x * step; base < old; base += (int64_t)gridDim.x * step) {
+        if (aligned && base + step <= old) {
+            const f32x4* p = reinterpret_cast<const f32x4*>(weights + base) + threadIdx.x;
+            f32x4 w[VECS];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int64_t i = base + 4 * (q * HIST_THREADS + (int)threadIdx.x);
-            if (aligned && i + 4 <= old) {
-                w[q] = *reinterpret_cast<const f32x4*>(weights + i);
-            } else {
+            for (int q = 0; q < VECS; ++q) w[q] = p[q * HIST_THREADS];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[q][j] = i + j < old ? weights[i + j] : 0.0f;
-            }
-        }
+            for (int q = 0; q < VECS; ++q)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int64_t i = base + 4 * (q * HIST_THREADS + (int)threadIdx.x);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t k = weight_key(w[q][j]);
-                const bool in = i + j < old && (PASS == 0 || (uint32_t)((uint64_t)k >> (shift + bits)) == prefix);
-                hist_add(h, (k >> shift) & ((1u << bits) - 1), in);
+                for (int j = 0; j < 4; ++j) add(w[q][j], true);
+        } else {
+            const int count = old - base < step ? (int)(old - base) : step;
+            for (int i0 = 0; i0 < count; i0 += HIST_THREADS) {
+                const int i = i0 + (int)threadIdx.x;
+                add(i < count ? weights[base + i] : 0.0f, i < count);
             }
         }
     }
+    if (count_zeros && zeros && (threadIdx.x & 63) == 0)
+        atomicAdd(own + ((ZERO >> shift) & ((1u << bits) - 1)) * HIST_COPIES, zeros);
     __syncthreads();
-    for (int b = threadIdx.x; b < HIST_BINS; b += HIST_THREADS)
-        if (h[b]) atomicAdd(&s->hist[PASS][b], h[b]);
+    for (int b = threadIdx.x; b < HIST_BINS; b += HIST_THREADS) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int c = 0; c < HIST_COPIES; ++c) n += h[b * HIST_COPIES + c];
+        if (n) atomicAdd(&s->hist[PASS][b], n);
+    }
 }
 
 __device__ __forceinline__ uint32_t block_sum_u32(uint32_t v, uint32_t* s_w) {
@@ -231,25 +232,51 @@ __device__ __forceinline__ RowBits row_bits(int64_t i, int64_t N, int64_t old, c
     return r;
 }
 
-// Per workgroup, a run of `tiles` tiles: rows above the threshold and rows that equal it.
+// Per workgroup, a run of `tiles` tiles: rows above the threshold and rows that equal it, counted per wave with ballots.
 __global__ void __launch_bounds__(SELECT_THREADS) select_count_kernel(int64_t N, int64_t old, int tiles,
                                                                       const float* __restrict__ weights,
                                                                       SelectState* __restrict__ s, uint2* __restrict__ counts) {
-    __shared__ uint32_t s_w[4];
+    __shared__ uint2 s_w[SELECT_THREADS / WAVE];
     const uint2 at = find_bin<2, SELECT_THREADS>(s);
     if (blockIdx.x == 0 && threadIdx.x == 0) s->at[3] = at;
     const bool aligned = ((uintptr_t)weights & 15) == 0;
     uint32_t above = 0, level = 0;
-    for (int t = 0; t < tiles; ++t) {
-        const int64_t i = ((int64_t)blockIdx.x * tiles + t) * SELECT_ROWS + 16 * (int)threadIdx.x;
-        if (i >= N) break;
-        const RowBits r = row_bits(i, N, old, weights, at.x, aligned);
-        above += (uint32_t)__popc(r.above);
-        level += (uint32_t)__popc(r.level);
+    auto add = [&](float w, bool valid) {
+        const uint32_t k = weight_key(w);
+        above += (uint32_t)__popcll(__ballot(valid && k > at.x));
+        level += (uint32_t)__popcll(__ballot(valid && k == at.x));
+    };
+    const int64_t begin = (int64_t)blockIdx.x * tiles * SELECT_ROWS;
+    int64_t end = begin + (int64_t)tiles * SELECT_ROWS;
+    if (end > N) end = N;
+    const int64_t stop = end < old ? end : old;   // the recent rows behind are kept unseen
+    int64_t base = begin;
+    if (aligned) {
+        for (; base + SELECT_ROWS <= stop; base += SELECT_ROWS) {
+            const f32x4* p = reinterpret_cast<const f32x4*>(weights + base) + threadIdx.x;
+            f32x4 w[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) w[q] = p[q * SELECT_THREADS];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) add(w[q][j], true);
+        }
     }
-    above = block_sum_u32(above, s_w);
-    level = block_sum_u32(level, s_w);
-    if (threadIdx.x == 0) counts[blockIdx.x] = make_uint2(above, level);
+    for (; base < stop; base += SELECT_THREADS) {
+        const int64_t i = base + (int)threadIdx.x;
+        add(i < stop ? weights[i] : 0.0f, i < stop);
+    }
+    if ((threadIdx.x & 63) == 0) s_w[threadIdx.x >> 6] = make_uint2(above, level);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint2 c = make_uint2(end > old ? (uint32_t)(end - (begin > old ? begin : old)) : 0u, 0u);
+        for (int w = 0; w < SELECT_THREADS / WAVE; ++w) {
+            c.x += s_w[w].x;
+            c.y += s_w[w].y;
+        }
+        counts[blockIdx.x] = c;
+    }
 }
 
 // The kept rows of a tile are gathered in LDS and leave in one run: a thread's own sixteen would be stored 64 bytes apart.
@@ -488,6 +515,17 @@ size_t evict_temp_bytes(int64_t N) {
     return align_up(sizeof(SelectState), 256) + SELECT_GROUPS * sizeof(uint2);
 }
 
+// One vector a thread while that gives every workgroup at most one step, four from there on.
+template <int PASS>
+static void launch_hist(int64_t old, const float* weights, SelectState* s, hipStream_t st) {
+    const int64_t steps = (old + 4 * HIST_THREADS - 1) / (4 * HIST_THREADS);
+    if (steps <= HIST_GROUPS)
+        hipLaunchKernelGGL((select_hist_kernel<PASS, 1>), dim3((unsigned)steps), dim3(HIST_THREADS), 0, st, old, weights, s);
+    else
+        hipLaunchKernelGGL((select_hist_kernel<PASS, 4>), dim3((unsigned)((steps + 3) / 4 < HIST_GROUPS ? (steps + 3) / 4 : HIST_GROUPS)),
+                           dim3(HIST_THREADS), 0, st, old, weights, s);
+}
+
 hipError_t launch_evict_select(int64_t N, const float* weights, int64_t budget, int64_t recent, int32_t* rows, void* temp,
                                hipStream_t st) {
     const int64_t keep = budget < N ? budget : N;
@@ -500,13 +538,13 @@ hipError_t launch_evict_select(int64_t N, const float* weights, int64_t budget, 
     const int64_t old = N - recent;
     SelectState* s = (SelectState*)temp;
     uint2* counts = (uint2*)((char*)temp + align_up(sizeof(SelectState), 256));
-    const int64_t steps = (old + HIST_STEP - 1) / HIST_STEP, all = (N + SELECT_ROWS - 1) / SELECT_ROWS;
+    const int64_t all = (N + SELECT_ROWS - 1) / SELECT_ROWS;
     const int tiles = (int)((all + SELECT_GROUPS - 1) / SELECT_GROUPS);
-    const dim3 hist((unsigned)(steps < HIST_GROUPS ? steps : HIST_GROUPS)), groups((unsigned)((all + tiles - 1) / tiles));
+    const dim3 groups((unsigned)((all + tiles - 1) / tiles));
     hipLaunchKernelGGL(select_clear_kernel, dim3(24), dim3(256), 0, st, s, (uint32_t)(keep - recent));
-    hipLaunchKernelGGL(select_hist_kernel<0>, hist, dim3(HIST_THREADS), 0, st, old, weights, s);
-    hipLaunchKernelGGL(select_hist_kernel<1>, hist, dim3(HIST_THREADS), 0, st, old, weights, s);
-    hipLaunchKernelGGL(select_hist_kernel<2>, hist, dim3(HIST_THREADS), 0, st, old, weights, s);
+    launch_hist<0>(old, weights, s, st);
+    launch_hist<1>(old, weights, s, st);
+    launch_hist<2>(old, weights, s, st);
     hipLaunchKernelGGL(select_count_kernel, groups, dim3(SELECT_THREADS), 0, st, N, old, tiles, weights, s, counts);
     hipLaunchKernelGGL(select_write_kernel, groups, dim3(SELECT_THREADS), 0, st, N, old, tiles, weights, s, counts, rows);
     return hipGetLastError();
