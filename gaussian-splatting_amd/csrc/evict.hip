@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(256) accumulate_weights_kernel(const WeightArg
     for (; v + 8 <= a.views; v += 8) {
         vec c[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) c[u] = *reinterpret_cast<const vec*>(a.contribution[v + u] + i);
+        for (int u = 0; u < 8; ++u) c[u] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(a.contribution[v + u] + i));
 #pragma unroll
         for (int u = 0; u < 8; ++u) s += c[u];
     }

@@ -13,6 +13,8 @@
 // vanish there.
 #include "kernels.h"
 
+#include <type_traits>
+
 namespace gs {
 
 constexpr int NORM_THREADS = 256;
@@ -156,14 +158,22 @@ __device__ __forceinline__ typename S::T block_join(typename S::T v) {
     return v;
 }
 
-template <typename S>
-__device__ __forceinline__ void add_vector(typename S::T& a, const uint4& v, int type) {
+// Calls f with the type as a constant: one copy of the loop for each, where a test per value would cost more than the sum.
+template <typename F>
+__device__ __forceinline__ void with_type(int type, F f) {
+    if (type == GSO_F32) f(std::integral_constant<int, GSO_F32>());
+    else if (type == GSO_BF16) f(std::integral_constant<int, GSO_BF16>());
+    else f(std::integral_constant<int, GSO_F16>());
+}
+
+template <typename S, int TYPE>
+__device__ __forceinline__ void add_vector(typename S::T& a, const uint4& v) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        if (type == GSO_F32) {
+        if (TYPE == GSO_F32) {
             S::add(a, __builtin_bit_cast(float, w[j]));
-        } else if (type == GSO_BF16) {
+        } else if (TYPE == GSO_BF16) {
             S::add(a, __builtin_bit_cast(float, w[j] << 16));
             S::add(a, __builtin_bit_cast(float, w[j] & 0xffff0000u));
         } else {
@@ -171,6 +181,22 @@ __device__ __forceinline__ void add_vector(typename S::T& a, const uint4& v, int
             S::add(a, f16_to_float((uint16_t)(w[j] >> 16)));
         }
     }
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint4 scale_vector(const uint4& v, float s) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (TYPE == GSO_F32) w[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, w[j]) * s);
+        else if (TYPE == GSO_BF16)
+            w[j] = (uint32_t)float_to_bf16(__builtin_bit_cast(float, w[j] << 16) * s) |
+                   (uint32_t)float_to_bf16(__builtin_bit_cast(float, w[j] & 0xffff0000u) * s) << 16;
+        else
+            w[j] = (uint32_t)float_to_f16(f16_to_float((uint16_t)w[j]) * s) |
+                   (uint32_t)float_to_f16(f16_to_float((uint16_t)(w[j] >> 16)) * s) << 16;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <bool ONCE>
@@ -202,8 +228,10 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_kernel(const NormTable t, u
                     v[u] = i >= lo && i < hi ? load_vector<ONCE>(c.base + 16 * i) : make_uint4(0, 0, 0, 0);   // zeros add nothing
                 }
             }
+            with_type(c.type, [&](auto type) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) add_vector<S>(a, v[u], c.type);
+                for (int u = 0; u < 4; ++u) add_vector<S, decltype(type)::value>(a, v[u]);
+            });
         }, [&](int x) {
             if (c.type == GSO_F32) S::add(a, *(const float*)(c.base + x));
             else if (c.type == GSO_BF16) S::add(a, bf16_to_float(*(const uint16_t*)(c.base + x)));
@@ -227,7 +255,13 @@ __global__ void __launch_bounds__(FINISH_THREADS) norm_finish_kernel(const uint6
                                                                      float* __restrict__ norm_out) {
     typedef Share<KIND> S;
     typename S::T a = S::zero();
-    for (int i = threadIdx.x; i < count; i += FINISH_THREADS) a = S::join(a, S::of(partial[i]));
+    for (int i = threadIdx.x; i < count; i += 4 * FINISH_THREADS) {
+        typename S::T v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = i + u * FINISH_THREADS < count ? S::of(partial[i + u * FINISH_THREADS]) : S::zero();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) a = S::join(a, v[u]);
+    }
     a = block_join<S, FINISH_THREADS>(a);
     if (threadIdx.x == 0) {
         const double norm = S::norm(a);
@@ -250,25 +284,15 @@ __global__ void __launch_bounds__(NORM_THREADS) scale_kernel(const NormTable t, 
             const int i = u * NORM_THREADS + (int)threadIdx.x;
             if (i >= lo && i < hi) v[u] = load_vector<true>(c.base + 16 * i);
         }
+        with_type(c.type, [&](auto type) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = u * NORM_THREADS + (int)threadIdx.x;
-            if (i >= lo && i < hi) {
-                uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (c.type == GSO_F32) w[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, w[j]) * s);
-                    else if (c.type == GSO_BF16)
-                        w[j] = (uint32_t)float_to_bf16(__builtin_bit_cast(float, w[j] << 16) * s) |
-                               (uint32_t)float_to_bf16(__builtin_bit_cast(float, w[j] & 0xffff0000u) * s) << 16;
-                    else
-                        w[j] = (uint32_t)float_to_f16(f16_to_float((uint16_t)w[j]) * s) |
-                               (uint32_t)float_to_f16(f16_to_float((uint16_t)(w[j] >> 16)) * s) << 16;
-                }
-                __builtin_nontemporal_store(__builtin_bit_cast(f32x4, make_uint4(w[0], w[1], w[2], w[3])),
-                                            reinterpret_cast<f32x4*>(c.base + 16 * i));
+            for (int u = 0; u < 4; ++u) {
+                const int i = u * NORM_THREADS + (int)threadIdx.x;
+                if (i >= lo && i < hi)
+                    __builtin_nontemporal_store(__builtin_bit_cast(f32x4, scale_vector<decltype(type)::value>(v[u], s)),
+                                                reinterpret_cast<f32x4*>(c.base + 16 * i));
             }
-        }
+        });
     }, [&](int x) {
         char* p = c.base + x;
         if (c.type == GSO_F32) *(float*)p = *(const float*)p * s;
@@ -449,7 +473,8 @@ hipError_t launch_grad_norm(int n, const void* const* grads, const int64_t* nume
                             bool read_again, void* temp, int* partials, hipStream_t st) {
     int count = 0;
     const hipError_t e = for_each_table(n, grads, numels, types, [&](const NormTable& t) {
-        const unsigned groups = t.chunks < (uint32_t)NORM_GROUPS ? t.chunks : (unsigned)NORM_GROUPS;
+        const uint32_t rounds = (t.chunks + NORM_GROUPS - 1) / NORM_GROUPS;   // the same number for every workgroup
+        const unsigned groups = (t.chunks + rounds - 1) / rounds;
         uint64_t* p = norm_partials(temp) + count;
         if (kind == 2) launch_norm<2>(t, read_again, groups, p, st);
         else if (kind == 1) launch_norm<1>(t, read_again, groups, p, st);

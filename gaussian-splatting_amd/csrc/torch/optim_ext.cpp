@@ -94,8 +94,10 @@ void check_disjoint(const Grads& g, const char* what) {
                     ": two gradients share memory (is a parameter listed twice?)");
 }
 
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+
 void check_may_wait(const char* what) {
-    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, what,
+    TORCH_CHECK(!capturing(), what,
                 ": error_if_nonfinite makes the host wait, which a stream capture does not allow");
 }
 
@@ -155,50 +157,73 @@ Tensor clip_grad_norm(const std::vector<Tensor>& params, double max_norm, double
     return r.value;
 }
 
-// Parameters with their moments, step sizes as the optimizer's groups hold them: scalars has six numbers per tensor,
-// (lr, beta1, beta2, eps, 1 - beta1^t, sqrt(1 - beta2^t)).  Tensors marked `idle` count in the norm and are not updated.
+// Parameters with gradients, their moments and step counts; scalars has four numbers per tensor, (lr, beta1, beta2, eps).
+// Tensors marked `idle` count in the norm and are not updated.  The step counts go up once nothing can fail any more.
 Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>& exp_avg,
-                    const std::vector<Tensor>& exp_avg_sq, const std::vector<double>& scalars, const std::vector<bool>& idle,
-                    const c10::optional<Tensor>& visible, double max_norm, double norm_type, bool error_if_nonfinite) {
+                    const std::vector<Tensor>& exp_avg_sq, const std::vector<Tensor>& steps,
+                    const std::vector<double>& scalars, const std::vector<bool>& idle, const c10::optional<Tensor>& visibility,
+                    double max_norm, double norm_type, bool error_if_nonfinite) {
     const char* what = "clipped_adam_step";
     const int kind = norm_kind(norm_type, what);
     const Grads g = collect(params, what);
     const size_t n = params.size();
-    TORCH_CHECK(g.own.size() == n && exp_avg.size() == n && exp_avg_sq.size() == n && scalars.size() == 6 * n &&
-                    idle.size() == n, what, ": inconsistent lists");
+    TORCH_CHECK(g.own.size() == n && exp_avg.size() == n && exp_avg_sq.size() == n && steps.size() == n &&
+                    scalars.size() == 4 * n && idle.size() == n, what, ": inconsistent lists");
     if (n == 0) return torch::zeros({});
+    torch::NoGradGuard no_grad;
     const c10::Device dev = g.own[0].device();
     c10::DeviceGuard guard(dev);
-    if (error_if_nonfinite) check_may_wait(what);
+    TORCH_CHECK(!capturing(), what, " cannot be captured into a graph: its bias correction follows the step count, which lives "
+                "on the host");
+    Tensor visible;
+    if (visibility) {
+        TORCH_CHECK(visibility->device() == dev, what, ": visibility must be on ", dev, ", got ", visibility->device());
+        visible = visibility->element_size() == 1 && !visibility->is_floating_point() ? visibility->contiguous()
+                                                                                      : visibility->ne(0).contiguous();
+    }
     std::vector<GsoAdamTensor> table;
     std::vector<Tensor> keep;
+    std::vector<size_t> counted;
     table.reserve(n);
     for (size_t i = 0; i < n; ++i) {
-        if (idle[i] || params[i].numel() == 0) continue;
-        for (const Tensor* t : {&params[i], &exp_avg[i], &exp_avg_sq[i]})
+        const Tensor& p = params[i];
+        for (const Tensor* t : {&p, &exp_avg[i], &exp_avg_sq[i]})
             TORCH_CHECK(t->device() == dev && t->scalar_type() == torch::kFloat32 && t->is_contiguous() &&
-                            t->sizes() == params[i].sizes(), what,
+                            t->sizes() == p.sizes(), what,
                         ": parameters and moments must be contiguous float32 tensors of one shape on the gradients' device");
         TORCH_CHECK(g.own[i].scalar_type() == torch::kFloat32, what, ": gradients must be float32");
-        keep.push_back(g.own[i].contiguous());
+        TORCH_CHECK(steps[i].numel() == 1 && steps[i].is_cpu() && steps[i].scalar_type() == torch::kFloat32, what,
+                    ": step counts must be float32 numbers on the host");
+        if (idle[i]) continue;
+        const int64_t rows = p.dim() > 0 ? p.size(0) : 1;
+        TORCH_CHECK(!visible.defined() || visible.numel() == rows, what, ": visibility must have one entry per Gaussian");
+        const double* s = &scalars[4 * i];
         GsoAdamTensor a;
-        a.param = params[i].data_ptr<float>();
+        a.lr = s[0]; a.beta1 = s[1]; a.beta2 = s[2]; a.eps = s[3];
+        a.bias_correction1 = a.bias_correction2_sqrt = 1.0;
+        if (!visible.defined()) {
+            const double t = (double)*steps[i].data_ptr<float>() + 1.0;
+            a.bias_correction1 = 1.0 - std::pow(a.beta1, t);
+            a.bias_correction2_sqrt = std::sqrt(1.0 - std::pow(a.beta2, t));
+            counted.push_back(i);
+        }
+        if (p.numel() == 0) continue;
+        keep.push_back(g.own[i].contiguous());
+        a.param = p.data_ptr<float>();
         a.grad = keep.back().data_ptr<float>();
         a.exp_avg = exp_avg[i].data_ptr<float>();
         a.exp_avg_sq = exp_avg_sq[i].data_ptr<float>();
-        a.rows = params[i].dim() > 0 ? params[i].size(0) : 1;
-        a.width = params[i].numel() / a.rows;
-        const double* s = &scalars[6 * i];
-        a.lr = s[0]; a.beta1 = s[1]; a.beta2 = s[2]; a.eps = s[3]; a.bias_correction1 = s[4]; a.bias_correction2_sqrt = s[5];
-        TORCH_CHECK(!visible || visible->numel() == a.rows, what, ": visibility must have one entry per Gaussian");
+        a.rows = rows;
+        a.width = p.numel() / rows;
         table.push_back(a);
     }
     void* st = stream_on(dev);
     Norm r = sums_of(g, kind, false, st, what);
     if (error_if_nonfinite) raise_if_nonfinite(r, kind, st, what);
-    check_rc(gso_adam_clipped((int)table.size(), table.data(), visible ? (const uint8_t*)visible->data_ptr() : nullptr, kind,
-                              max_norm, r.temp.data_ptr(), r.partials, r.value.data_ptr<float>(), st),
+    check_rc(gso_adam_clipped((int)table.size(), table.data(), visible.defined() ? (const uint8_t*)visible.data_ptr() : nullptr,
+                              kind, max_norm, r.temp.data_ptr(), r.partials, r.value.data_ptr<float>(), st),
              what);
+    for (size_t i : counted) *steps[i].data_ptr<float>() += 1.0f;
     return r.value;
 }
 

@@ -142,65 +142,41 @@ def clipped_adam_step(optimizer, max_norm, visibility=None, N=None, norm_type=2.
         raise RuntimeError(f"{what} needs a torch.optim.Adam, got {type(optimizer).__name__}")
     if not float(max_norm) >= 0.0:
         raise RuntimeError(f"{what}: max_norm must not be negative or NaN, got {max_norm}")
-    vis = None
-    if visibility is not None:
-        vis = visibility.to(torch.uint8) if visibility.dtype not in (torch.uint8, torch.bool) else visibility
-        vis = vis.contiguous()
-    entries, device = [], None
+    entries = []
     for group in optimizer.param_groups:
         if group["weight_decay"] or group["amsgrad"] or group["maximize"] or group["capturable"] or group["differentiable"]:
             raise RuntimeError(f"{what}: weight_decay, amsgrad, maximize, capturable and differentiable are not supported")
         beta1, beta2 = group["betas"]
-        lr, eps = float(group["lr"]), float(group["eps"])
+        scalars = (float(group["lr"]), float(beta1), float(beta2), float(group["eps"]))
         for p in group["params"]:
             if p.grad is None:
                 continue
             if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
                 raise RuntimeError(f"{what} needs contiguous float32 GPU parameters (there is no CPU path)")
-            if device is None:
-                device = p.device
-            rows = p.shape[0] if p.dim() > 0 else 1
-            idle = False
-            if vis is not None:
-                idle = N is not None and rows != N   # a group that is not per-Gaussian takes no sparse step
-                if not idle and vis.numel() != rows:
-                    raise RuntimeError("visibility must have one entry per Gaussian")
-            entries.append((p, lr, beta1, beta2, eps, idle))
-    if vis is not None and device is not None and vis.device != device:
-        raise RuntimeError(f"{what}: visibility must be on {device}, got {vis.device}")
-    if device is not None:
-        with torch.cuda.device(device):
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"{what} cannot be captured into a graph: its bias correction follows the step count, "
-                                   "which lives on the host")
-    params, m, v, scalars, idles, fresh, counts = [], [], [], [], [], [], []
-    for p, lr, beta1, beta2, eps, idle in entries:
-        st = optimizer.state[p]
-        if len(st) == 0:
-            st["step"] = torch.tensor(0.0, dtype=torch.float32)
-            st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            fresh.append(p)
-        params.append(p)
-        m.append(st["exp_avg"])
-        v.append(st["exp_avg_sq"])
-        idles.append(idle)
-        if idle or vis is not None:
-            scalars += (lr, beta1, beta2, eps, 1.0, 1.0)
-        else:
-            t = float(st["step"]) + 1.0
-            counts.append(st)
-            scalars += (lr, beta1, beta2, eps, 1.0 - beta1 ** t, math.sqrt(1.0 - beta2 ** t))
+            # a group that is not per-Gaussian takes no sparse step
+            idle = visibility is not None and N is not None and (p.shape[0] if p.dim() > 0 else 1) != N
+            entries.append((p, scalars, idle))
+    params, m, v, steps, flat, idles, fresh = [], [], [], [], [], [], []
     try:
-        norm = _host().clipped_adam(params, m, v, scalars, idles, vis, float(max_norm), float(norm_type),
+        for p, scalars, idle in entries:
+            st = optimizer.state[p]
+            if len(st) == 0:
+                fresh.append(p)
+                st["step"] = torch.tensor(0.0, dtype=torch.float32)
+                st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            params.append(p)
+            m.append(st["exp_avg"])
+            v.append(st["exp_avg_sq"])
+            steps.append(st["step"])
+            flat += scalars
+            idles.append(idle)
+        return _host().clipped_adam(params, m, v, steps, flat, idles, visibility, float(max_norm), float(norm_type),
                                     bool(error_if_nonfinite))
     except Exception:
         for p in fresh:
             del optimizer.state[p]
         raise
-    for st in counts:
-        st["step"] += 1
-    return norm
 
 
 @torch.no_grad()
