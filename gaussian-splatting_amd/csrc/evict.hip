@@ -157,8 +157,11 @@ __global__ void __launch_bounds__(HIST_THREADS) select_hist_kernel(int64_t old, 
     uint32_t zeros = 0;
     auto add = [&](float w, bool valid) {
         const uint32_t k = weight_key(w);
-        zeros += (uint32_t)__popcll(__ballot(valid && k == ZERO));
-        const bool in = valid && k != ZERO && (PASS == 0 || (uint32_t)((uint64_t)k >> (shift + bits)) == prefix);
+        bool in = valid && (PASS == 0 || (uint32_t)((uint64_t)k >> (shift + bits)) == prefix);
+        if (count_zeros) {
+            zeros += (uint32_t)__popcll(__ballot(valid && k == ZERO));
+            in = in && k != ZERO;
+        }
         if (in) atomicAdd(own + ((k >> shift) & ((1u << bits) - 1)) * HIST_COPIES, 1u);
     };
     const bool aligned = ((uintptr_t)weights & 15) == 0;
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(HIST_THREADS) select_hist_kernel(int64_t old, 
             }
         }
     }
-    if (count_zeros && zeros && (threadIdx.x & 63) == 0)
+    if (zeros && (threadIdx.x & 63) == 0)
         atomicAdd(own + ((ZERO >> shift) & ((1u << bits) - 1)) * HIST_COPIES, zeros);
     __syncthreads();
     for (int b = threadIdx.x; b < HIST_BINS; b += HIST_THREADS) {
@@ -519,11 +522,14 @@ size_t evict_temp_bytes(int64_t N) {
 template <int PASS>
 static void launch_hist(int64_t old, const float* weights, SelectState* s, hipStream_t st) {
     const int64_t steps = (old + 4 * HIST_THREADS - 1) / (4 * HIST_THREADS);
-    if (steps <= HIST_GROUPS)
+    if (steps <= HIST_GROUPS) {
         hipLaunchKernelGGL((select_hist_kernel<PASS, 1>), dim3((unsigned)steps), dim3(HIST_THREADS), 0, st, old, weights, s);
-    else
-        hipLaunchKernelGGL((select_hist_kernel<PASS, 4>), dim3((unsigned)((steps + 3) / 4 < HIST_GROUPS ? (steps + 3) / 4 : HIST_GROUPS)),
+    } else {
+        constexpr int VECS = 4;
+        const int64_t wide = (steps + VECS - 1) / VECS;
+        hipLaunchKernelGGL((select_hist_kernel<PASS, VECS>), dim3((unsigned)(wide < HIST_GROUPS ? wide : HIST_GROUPS)),
                            dim3(HIST_THREADS), 0, st, old, weights, s);
+    }
 }
 
 hipError_t launch_evict_select(int64_t N, const float* weights, int64_t budget, int64_t recent, int32_t* rows, void* temp,
