@@ -22,6 +22,11 @@ void* stream_on(const c10::Device& dev) {
     return (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
 }
 
+// What a kernel has written through a pointer counts as an in-place change for autograd.
+void changed(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 int norm_kind(double p, const char* what) {
     TORCH_CHECK(p == 1.0 || p == 2.0 || (std::isinf(p) && p > 0), what, ": norm_type must be 1, 2 or inf, got ", p);
     return std::isinf(p) ? 0 : (int)p;
@@ -152,10 +157,14 @@ Tensor clip_grad_norm(const std::vector<Tensor>& params, double max_norm, double
                             r.value.data_ptr<float>(), st),
              what);
     torch::NoGradGuard no_grad;
-    for (size_t i = 0; i < g.own.size(); ++i)
+    for (size_t i = 0; i < g.own.size(); ++i) {
         if (!g.packed[i].is_same(g.own[i])) g.own[i].copy_(g.packed[i]);
+        else changed(g.own[i]);
+    }
     return r.value;
 }
+
+bool on_host(const Tensor& step) { return step.is_cpu() && step.scalar_type() == torch::kFloat32; }
 
 // Parameters with gradients, their moments and step counts; scalars has four numbers per tensor, (lr, beta1, beta2, eps).
 // Tensors marked `idle` count in the norm and are not updated.  The step counts go up once nothing can fail any more.
@@ -192,8 +201,7 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
                             t->sizes() == p.sizes(), what,
                         ": parameters and moments must be contiguous float32 tensors of one shape on the gradients' device");
         TORCH_CHECK(g.own[i].scalar_type() == torch::kFloat32, what, ": gradients must be float32");
-        TORCH_CHECK(steps[i].numel() == 1 && steps[i].is_cpu() && steps[i].scalar_type() == torch::kFloat32, what,
-                    ": step counts must be float32 numbers on the host");
+        TORCH_CHECK(steps[i].numel() == 1, what, ": a step count must be one number");
         if (idle[i]) continue;
         const int64_t rows = p.dim() > 0 ? p.size(0) : 1;
         TORCH_CHECK(!visible.defined() || visible.numel() == rows, what, ": visibility must have one entry per Gaussian");
@@ -202,7 +210,8 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
         a.lr = s[0]; a.beta1 = s[1]; a.beta2 = s[2]; a.eps = s[3];
         a.bias_correction1 = a.bias_correction2_sqrt = 1.0;
         if (!visible.defined()) {
-            const double t = (double)*steps[i].data_ptr<float>() + 1.0;
+            // a count that a checkpoint has brought to the GPU makes the host wait, as it does in FusedGaussianAdam.step
+            const double t = (on_host(steps[i]) ? (double)*steps[i].data_ptr<float>() : steps[i].item<double>()) + 1.0;
             a.bias_correction1 = 1.0 - std::pow(a.beta1, t);
             a.bias_correction2_sqrt = std::sqrt(1.0 - std::pow(a.beta2, t));
             counted.push_back(i);
@@ -223,7 +232,16 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
     check_rc(gso_adam_clipped((int)table.size(), table.data(), visible.defined() ? (const uint8_t*)visible.data_ptr() : nullptr,
                               kind, max_norm, r.temp.data_ptr(), r.partials, r.value.data_ptr<float>(), st),
              what);
-    for (size_t i : counted) *steps[i].data_ptr<float>() += 1.0f;
+    for (size_t i : counted) {
+        if (on_host(steps[i])) *steps[i].data_ptr<float>() += 1.0f;
+        else steps[i].add_(1);
+    }
+    for (size_t i = 0; i < n; ++i) {
+        if (idle[i]) continue;
+        changed(params[i]);
+        changed(exp_avg[i]);
+        changed(exp_avg_sq[i]);
+    }
     return r.value;
 }
 
@@ -254,6 +272,7 @@ void accumulate_weights(const Tensor& weights, const std::vector<Tensor>& contri
     c10::DeviceGuard guard(weights.device());
     check_rc(gso_accumulate_weights(N, weights.data_ptr<float>(), (int)ptr.size(), ptr.data(), o, decay,
                                     stream_on(weights.device())), what);
+    changed(weights);
 }
 
 Tensor evict_select(const Tensor& weights, int64_t budget, int64_t recent) {

@@ -108,8 +108,9 @@ def grad_norm(parameters, norm_type=2.0):
 
     Parameters without a gradient are left out (without any: a CPU zero, as torch.nn.utils.clip_grad_norm_ gives).
     Gradients are float32, bfloat16 or float16 GPU tensors of one device, of mixed types and any sizes.  Sums are held
-    in 64 bits and added in a fixed order, so the result does not depend on the run, and replicas that hold the same
-    gradients (after `gsdp.GradReducer`) get the same bits.  A NaN makes the norm NaN."""
+    in 64 bits and added in an order that the tensors' sizes and their addresses modulo 16 fix, so the result does not
+    depend on the run, and replicas with the same gradients in the same layout (a `ParamGradSink` each, after
+    `gsdp.GradReducer`) get the same bits.  A NaN makes the norm NaN; one beyond float32 is infinite."""
     return _host().grad_norm(_tensors(parameters), float(norm_type))
 
 
@@ -135,8 +136,9 @@ def clipped_adam_step(optimizer, max_norm, visibility=None, N=None, norm_type=2.
 
     The norm counts every gradient of the optimizer, also those of groups that take no sparse step because their rows
     are not N.  Needs contiguous float32 GPU parameters and plain Adam groups (no weight decay, amsgrad, maximize,
-    capturable); cannot be captured into a graph (the bias correction is a number of the host).  error_if_nonfinite:
-    the host waits for the norm and a RuntimeError leaves parameters, moments and step counts as they were."""
+    capturable, fused); cannot be captured into a graph (the bias correction is a number of the host).  Hooks that were
+    registered on `step` do not run.  error_if_nonfinite: the host waits for the norm and a RuntimeError leaves
+    parameters, moments and step counts as they were."""
     what = "clipped_adam_step"
     if not isinstance(optimizer, torch.optim.Adam):
         raise RuntimeError(f"{what} needs a torch.optim.Adam, got {type(optimizer).__name__}")
@@ -144,8 +146,8 @@ def clipped_adam_step(optimizer, max_norm, visibility=None, N=None, norm_type=2.
         raise RuntimeError(f"{what}: max_norm must not be negative or NaN, got {max_norm}")
     entries = []
     for group in optimizer.param_groups:
-        if group["weight_decay"] or group["amsgrad"] or group["maximize"] or group["capturable"] or group["differentiable"]:
-            raise RuntimeError(f"{what}: weight_decay, amsgrad, maximize, capturable and differentiable are not supported")
+        if any(group.get(k) for k in ("weight_decay", "amsgrad", "maximize", "capturable", "differentiable", "fused")):
+            raise RuntimeError(f"{what}: weight_decay, amsgrad, maximize, capturable, differentiable and fused are not supported")
         beta1, beta2 = group["betas"]
         scalars = (float(group["lr"]), float(beta1), float(beta2), float(group["eps"]))
         for p in group["params"]:

@@ -345,3 +345,46 @@ def test_a_training_run_within_its_bounds():
             # which the bound of the update, lr / sqrt(1 - beta2), covers: 0.032 per step) and one of the parameter
             bound = 6 * (0.032 * 40 * U) + 6 * U * plain[k][0].abs()
             assert bool(((params[k].double() - plain[k][0]).abs() <= bound)[sure].all()), k
+
+
+@pytest.mark.parametrize("shape,dtype", [((40, 40001), torch.float32), ((40, 40000), torch.float32), ((33, 70001), torch.bfloat16),
+                                         ((33, 33333), torch.int8), ((17, 20002), torch.float32)])
+def test_wide_rows(shape, dtype):
+    import gsplat_optim as G
+    t = (torch.randn(shape, device="cuda") * 40).to(dtype)
+    rows, (k,) = G.evict_rows(torch.rand(shape[0], device="cuda"), shape[0] - 9, 0, [t])
+    assert torch.equal(k, t[rows.long()])
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 3, 4, 8])
+@pytest.mark.parametrize("row_bytes,pitch", [(12, 12), (16, 16), (16, 20), (5, 5), (6, 8), (180, 180), (4, 4), (1, 1), (1, 3), (64, 0)])
+def test_c_abi_copies_to_any_address(offset, row_bytes, pitch):
+    """Through the C ABI the copy may start anywhere; what lies around it stays."""
+    import ctypes as C
+    from _gsplat_lib import check, lib
+    N, K = 700, 411
+    gen = torch.Generator(device="cuda").manual_seed(offset)
+    src = torch.randint(0, 250, (N * max(pitch, 1) + row_bytes + 64,), device="cuda", generator=gen, dtype=torch.int32).to(torch.uint8)
+    dst = torch.full((K * row_bytes + 64,), 255, dtype=torch.uint8, device="cuda")
+    rows = torch.randperm(N, device="cuda", generator=gen)[:K].sort().values.to(torch.int32)
+    entry = (C.c_int64 * 4)(src.data_ptr() + offset, dst.data_ptr() + offset, row_bytes, pitch)
+    check(lib().gso_gather_rows_multi(1, C.addressof(entry), rows.data_ptr(), K, torch.cuda.current_stream().cuda_stream), "gather")
+    at = offset + rows.long()[:, None] * pitch + torch.arange(row_bytes, device="cuda")[None]
+    torch.cuda.synchronize()
+    assert torch.equal(dst[offset:offset + K * row_bytes].view(K, row_bytes), src[at])
+    assert bool((dst[:offset] == 255).all()) and bool((dst[offset + K * row_bytes:] == 255).all())
+
+
+def test_two_evictions_at_once_on_two_streams():
+    import gsplat_optim as G
+    ws = [torch.rand(200_003, device="cuda") for _ in range(2)]
+    ts = [torch.randn(200_003, 45, device="cuda") for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in ws]
+    torch.cuda.synchronize()
+    out = []
+    for w, t, st in zip(ws, ts, streams):
+        with torch.cuda.stream(st):
+            out.append(G.evict_rows(w, 150_000, 1000, [t]))
+    torch.cuda.synchronize()
+    for w, t, (rows, kept) in zip(ws, ts, out):
+        assert np.array_equal(rows.cpu().numpy(), _reference(w, 150_000, 1000)) and torch.equal(kept[0], t[rows.long()])

@@ -386,3 +386,96 @@ def test_the_norm_is_the_same_bits_in_every_run():
     first = G.grad_norm(params)
     for _ in range(20):
         assert torch.equal(first, G.grad_norm(params))
+
+
+def test_in_place_changes_are_seen_by_autograd():
+    import gsplat_optim as G
+    p = torch.nn.Parameter(torch.ones(100, 3, device="cuda"))
+    opt = G.FusedGaussianAdam([p], lr=0.1)
+    p.grad = torch.ones_like(p)
+    g0, p0 = p.grad._version, p._version
+    G.clip_grad_norm_(p, 0.1)
+    assert p.grad._version > g0
+    y = (p * p).sum()                 # keeps p for its backward
+    opt.clipped_step(1.0)
+    assert p._version > p0
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    w, c = torch.zeros(5, device="cuda"), torch.ones(5, device="cuda")
+    w0 = w._version
+    G.accumulate_weights(w, c)
+    assert w._version > w0
+    with torch.inference_mode():
+        G.accumulate_weights(torch.zeros(5, device="cuda"), c)
+
+
+def test_step_counts_of_a_checkpoint_loaded_to_the_gpu():
+    import gsplat_optim as G
+    a, b = _optimizer(50, G.FusedGaussianAdam), _optimizer(50, G.FusedGaussianAdam)
+    for st in a.state.values():
+        st["step"] = st["step"].cuda()
+    a.clipped_step(0.01)
+    b.clipped_step(0.01)
+    for x, y in zip(_dump(a), _dump(b)):
+        assert torch.equal(x, y)
+    p = torch.nn.Parameter(torch.ones(4, device="cuda"))
+    p.grad = torch.ones_like(p)
+    with pytest.raises(RuntimeError, match="not supported"):
+        G.clipped_adam_step(torch.optim.Adam([p], fused=True), 1.0)
+
+
+@pytest.mark.parametrize("width", [1, 2, 3, 7, 45, 1000, 4097, 8191, 8192, 9001])
+@pytest.mark.parametrize("sparse", [False, True])
+def test_rows_of_any_width_and_parameters_at_any_address(width, sparse):
+    """Against clip_grad_norm_ and FusedGaussianAdam.step, which share no kernel with it; NaN around the tensors shows
+    an access beyond them."""
+    import gsplat_optim as G
+    N = max(3, 30000 // width)
+    gen = torch.Generator(device="cuda").manual_seed(width)
+    vis = torch.rand(N, device="cuda", generator=gen) < 0.4 if sparse else None
+
+    def make(off):
+        bufs = [torch.full((N * width + 16,), math.nan, device="cuda") for _ in range(4)]
+        views = [b[off:off + N * width].view(N, width) for b in bufs]
+        g2 = torch.Generator(device="cuda").manual_seed(7)
+        for v in views:
+            v.copy_(torch.randn(N, width, device="cuda", generator=g2))
+        views[3].square_()
+        p = torch.nn.Parameter(views[0])
+        p.grad = views[1]
+        opt = G.FusedGaussianAdam([{"params": [p], "lr": 0.1, "name": "xyz"}], eps=1e-15)
+        opt.state[p] = {"step": torch.tensor(4.0), "exp_avg": views[2], "exp_avg_sq": views[3]}
+        return bufs, p, opt
+    ref = None
+    for off in (0, 1, 2, 3, 4):
+        bufs, p, opt = make(off)
+        opt.clipped_step(0.5, vis, N if sparse else None)
+        got = [p.detach().clone(), opt.state[p]["exp_avg"].clone(), opt.state[p]["exp_avg_sq"].clone()]
+        for b in bufs:
+            assert bool(b[:off].isnan().all()) and bool(b[off + N * width:].isnan().all())
+            assert not bool(b[off:off + N * width].isnan().any())
+        if off == 0:
+            _, q, two = make(0)
+            G.clip_grad_norm_(q, 0.5)
+            two.step(vis, N if sparse else None)
+            assert all(torch.equal(x, y) for x, y in zip(got, (q.detach(), two.state[q]["exp_avg"], two.state[q]["exp_avg_sq"])))
+            ref = got
+        else:    # another address: the norm's sum runs in another order, one rounding of the coefficient apart at most
+            for x, y in zip(got, ref):
+                assert torch.allclose(x, y, rtol=1e-5, atol=1e-6)
+
+
+def test_two_calls_at_once_on_two_streams():
+    import gsplat_optim as G
+    sets = [_make([1 << 20, 333, 70001], [torch.float32, torch.bfloat16], seed=k) for k in range(2)]
+    want = [[g.clone() for g in s] for s in sets]
+    norms = [G.clip_grad_norm_(_params(w), 1.0) for w in want]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for s, st in zip(sets, streams):
+        with torch.cuda.stream(st):
+            got.append(G.clip_grad_norm_(_params(s), 1.0))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert torch.equal(got[k], norms[k]) and all(torch.equal(a, b) for a, b in zip(sets[k], want[k]))
