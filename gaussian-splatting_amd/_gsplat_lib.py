@@ -167,13 +167,12 @@ def lib():
     L.gso_norm_temp_bytes.restype = C.c_size_t
     L.gso_norm_temp_bytes.argtypes = [C.c_int]
     L.gso_grad_norm.restype = C.c_int
-    L.gso_grad_norm.argtypes = [C.c_int, _vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_size_t, _vp, _vp]
-    L.gso_norm_finish.restype = C.c_int
-    L.gso_norm_finish.argtypes = [_vp, C.c_int, C.c_int, _vp, _vp]
+    L.gso_grad_norm.argtypes = [C.c_int, _vp, _vp, _vp, C.c_int, _vp, C.c_size_t, _vp, _vp]
     L.gso_clip_grads.restype = C.c_int
-    L.gso_clip_grads.argtypes = [C.c_int, _vp, _vp, _vp, C.c_int, C.c_double, _vp, C.c_int, _vp, _vp]
+    L.gso_clip_grads.argtypes = [C.c_int, _vp, _vp, _vp, C.c_int, C.c_double, C.c_int, _vp, C.c_size_t, _vp, _vp]
     L.gso_adam_clipped.restype = C.c_int
-    L.gso_adam_clipped.argtypes = [C.c_int, _vp, _vp, C.c_int, C.c_double, _vp, C.c_int, _vp, _vp]
+    L.gso_adam_clipped.argtypes = [C.c_int, _vp, _vp, _vp, C.c_int, _vp, _vp, C.c_int, C.c_double, C.c_int, _vp,
+                                   C.c_size_t, _vp, _vp]
     L.gso_accumulate_weights.restype = C.c_int
     L.gso_accumulate_weights.argtypes = [C.c_int64, _vp, C.c_int, _vp, _vp, C.c_double, _vp]
     L.gso_evict_temp_bytes.restype = C.c_size_t
@@ -202,7 +201,7 @@ EXPORTED = ("gsr_geom_bytes", "gsr_image_bytes", "gsr_binning_bytes", "gsr_backw
             "gss_ssim_backward", "gss_loss_partial_floats", "gss_l1_ssim_loss_forward", "gss_l1_ssim_loss_backward",
             "gss_l1_partial_floats", "gss_l1_loss_forward", "gss_l1_loss_backward",
             "gso_adam_update", "gso_densify_stats", "gso_densify_select", "gso_mark_nonzero", "gso_prune_mask", "gso_split_children", "gso_compact_temp_bytes", "gso_compact_map",
-            "gso_gather_rows", "gso_norm_temp_bytes", "gso_grad_norm", "gso_norm_finish", "gso_clip_grads",
+            "gso_gather_rows", "gso_norm_temp_bytes", "gso_grad_norm", "gso_clip_grads",
             "gso_adam_clipped", "gso_accumulate_weights", "gso_evict_temp_bytes", "gso_evict_select",
             "gso_gather_rows_multi", "gsr_status_string", "gsr_struct_bytes")
 

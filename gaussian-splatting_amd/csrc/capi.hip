@@ -663,34 +663,37 @@ static bool norm_args_ok(int n, const void* const* grads, const int64_t* numels,
 
 size_t gso_norm_temp_bytes(int n) { return n < 0 ? 0 : norm_temp_bytes(n); }
 
-int gso_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type, int read_again,
-                  void* temp, size_t temp_bytes, int* partials, void* stream) {
-    if (!partials || !temp || ((uintptr_t)temp & 7u) != 0) return GSR_ERR_ARG;
+// What the three calls below have in common.
+static int check_norm_args(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type,
+                           const void* temp, size_t temp_bytes, const float* norm) {
+    if (!norm || !temp || ((uintptr_t)temp & 7u) != 0) return GSR_ERR_ARG;
     if (!norm_args_ok(n, grads, numels, types, norm_type)) return GSR_ERR_ARG;
     if (!norm_fits(n, numels)) return GSR_ERR_OVERFLOW;
-    if (temp_bytes < norm_temp_bytes(n)) return GSR_ERR_BUFFER;
-    return hip_status(launch_grad_norm(n, grads, numels, types, norm_type, read_again != 0, temp, partials,
-                                       (hipStream_t)stream));
+    return temp_bytes < norm_temp_bytes(n) ? GSR_ERR_BUFFER : GSR_OK;
 }
 
-int gso_norm_finish(void* temp, int partials, int norm_type, float* norm, void* stream) {
-    if (!temp || !norm || partials < 0 || norm_type < 0 || norm_type > 2) return GSR_ERR_ARG;
-    return hip_status(launch_norm_finish(temp, partials, norm_type, 0.0, norm, (hipStream_t)stream));
+int gso_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type, void* temp,
+                  size_t temp_bytes, float* norm, void* stream) {
+    const int rc = check_norm_args(n, grads, numels, types, norm_type, temp, temp_bytes, norm);
+    if (rc != GSR_OK) return rc;
+    return hip_status(launch_grad_norm(n, grads, numels, types, norm_type, temp, norm, (hipStream_t)stream));
 }
 
 int gso_clip_grads(int n, void* const* grads, const int64_t* numels, const int* types, int norm_type, double max_norm,
-                   void* temp, int partials, float* norm, void* stream) {
-    if (!temp || !norm || partials < 0 || !(max_norm >= 0.0)) return GSR_ERR_ARG;
-    if (!norm_args_ok(n, (const void* const*)grads, numels, types, norm_type)) return GSR_ERR_ARG;
-    if (!norm_fits(n, numels)) return GSR_ERR_OVERFLOW;
-    return hip_status(launch_clip_grads(n, grads, numels, types, norm_type, max_norm, temp, partials, norm,
+                   int norm_known, void* temp, size_t temp_bytes, float* norm, void* stream) {
+    const int rc = check_norm_args(n, (const void* const*)grads, numels, types, norm_type, temp, temp_bytes, norm);
+    if (rc != GSR_OK) return rc;
+    if (!(max_norm >= 0.0)) return GSR_ERR_ARG;
+    return hip_status(launch_clip_grads(n, grads, numels, types, norm_type, max_norm, norm_known != 0, temp, norm,
                                         (hipStream_t)stream));
 }
 
-int gso_adam_clipped(int n, const GsoAdamTensor* tensors, const uint8_t* visible, int norm_type, double max_norm,
-                     void* temp, int partials, float* norm, void* stream) {
-    if (n < 0 || (n > 0 && !tensors) || !temp || !norm || partials < 0 || !(max_norm >= 0.0)) return GSR_ERR_ARG;
-    if (norm_type < 0 || norm_type > 2) return GSR_ERR_ARG;
+int gso_adam_clipped(int ngrads, const void* const* grads, const int64_t* numels, const int* types, int n,
+                     const GsoAdamTensor* tensors, const uint8_t* visible, int norm_type, double max_norm, int norm_known,
+                     void* temp, size_t temp_bytes, float* norm, void* stream) {
+    const int rc = check_norm_args(ngrads, grads, numels, types, norm_type, temp, temp_bytes, norm);
+    if (rc != GSR_OK) return rc;
+    if (n < 0 || (n > 0 && !tensors) || !(max_norm >= 0.0)) return GSR_ERR_ARG;
     for (int i = 0; i < n; ++i) {
         const GsoAdamTensor& a = tensors[i];
         if (a.rows < 0 || a.width <= 0) return GSR_ERR_ARG;
@@ -701,8 +704,8 @@ int gso_adam_clipped(int n, const GsoAdamTensor* tensors, const uint8_t* visible
             return GSR_ERR_ARG;
         if (!(a.bias_correction1 > 0.0) || !(a.bias_correction2_sqrt > 0.0)) return GSR_ERR_ARG;
     }
-    return hip_status(launch_adam_clipped(n, tensors, visible, norm_type, max_norm, temp, partials, norm,
-                                          (hipStream_t)stream));
+    return hip_status(launch_adam_clipped(ngrads, grads, numels, types, n, tensors, visible, norm_type, max_norm,
+                                          norm_known != 0, temp, norm, (hipStream_t)stream));
 }
 
 int gso_accumulate_weights(int64_t N, float* weights, int views, const float* const* contributions, const float* opacity,

@@ -104,18 +104,16 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {   // inclusive
     return v;
 }
 
-// The bin of pass PASS that holds the need-th largest key, and how many of it are needed: every workgroup finds it for
-// itself from the finished histogram, which saves a launch between the passes.
+// The bin of a finished histogram (of pass PASS) that holds the at.y-th largest key, and how many of it are needed.
 template <int PASS, int THREADS>
-__device__ __forceinline__ uint2 find_bin(const SelectState* __restrict__ s) {
+__device__ __forceinline__ uint2 find_bin(const uint32_t* hist, uint2 at) {
     constexpr int PER = HIST_BINS / THREADS;
     __shared__ uint32_t s_w[THREADS / WAVE];
     __shared__ uint2 s_found;
-    const uint2 at = s->at[PASS];
     uint32_t c[PER], own = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {   // thread 0 has the highest bins
-        c[j] = s->hist[PASS][HIST_BINS - 1 - ((int)threadIdx.x * PER + j)];
+        c[j] = hist[HIST_BINS - 1 - ((int)threadIdx.x * PER + j)];
         own += c[j];
     }
     const uint32_t incl = wave_scan_u32(own);
@@ -146,7 +144,9 @@ __global__ void __launch_bounds__(HIST_THREADS) select_hist_kernel(int64_t old, 
     for (int b = threadIdx.x; b < HIST_BINS * HIST_COPIES; b += HIST_THREADS) h[b] = 0;
     uint32_t prefix = 0;
     if (PASS > 0) {
-        const uint2 at = find_bin<(PASS > 0 ? PASS - 1 : 0), HIST_THREADS>(s);
+        // every workgroup finds the bin of the pass before for itself, which saves a launch between the passes
+        constexpr int BEFORE = PASS > 0 ? PASS - 1 : 0;
+        const uint2 at = find_bin<BEFORE, HIST_THREADS>(s->hist[BEFORE], s->at[BEFORE]);
         prefix = at.x;
         if (blockIdx.x == 0 && threadIdx.x == 0) s->at[PASS] = at;
     } else {
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_count_kernel(int64_t N,
                                                                       const float* __restrict__ weights,
                                                                       SelectState* __restrict__ s, uint2* __restrict__ counts) {
     __shared__ uint2 s_w[SELECT_THREADS / WAVE];
-    const uint2 at = find_bin<2, SELECT_THREADS>(s);
+    const uint2 at = find_bin<2, SELECT_THREADS>(s->hist[2], s->at[2]);
     if (blockIdx.x == 0 && threadIdx.x == 0) s->at[3] = at;
     const bool aligned = ((uintptr_t)weights & 15) == 0;
     uint32_t above = 0, level = 0;
@@ -335,6 +335,70 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_write_kernel(int64_t N,
         above += tile_all & 0xffffu;
         level = level_end;
         __syncthreads();
+    }
+}
+
+// The whole selection in one workgroup, the keys in registers: one launch, which is what a small model's costs.
+constexpr int SMALL_THREADS = 1024;
+constexpr int SMALL_PER = 8;
+constexpr int SMALL_ROWS = SMALL_PER * SMALL_THREADS;
+template <int PASS>
+__device__ __forceinline__ uint2 small_pass(uint32_t* h, const uint32_t (&key)[SMALL_PER], uint32_t valid, uint2 at) {
+    constexpr int shift = pass_shift(PASS), bits = pass_bits(PASS);
+    for (int b = threadIdx.x; b < HIST_BINS; b += SMALL_THREADS) h[b] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < SMALL_PER; ++j) {
+        const bool in = (valid >> j & 1u) && (PASS == 0 || (uint32_t)((uint64_t)key[j] >> (shift + bits)) == at.x);
+        const uint32_t bin = (key[j] >> shift) & ((1u << bits) - 1);
+        // the lanes that share the first active lane's bin are added at once: weights repeat
+        const uint64_t act = __ballot(in);
+        if (act == 0) continue;
+        const int leader = __builtin_ctzll(act);
+        const bool same = in && bin == (uint32_t)__builtin_amdgcn_readlane((int)bin, leader);
+        const uint64_t m = __ballot(same);
+        if ((int)(threadIdx.x & 63) == leader) atomicAdd(&h[bin], (uint32_t)__popcll(m));
+        else if (in && !same) atomicAdd(&h[bin], 1u);
+    }
+    __syncthreads();
+    return find_bin<PASS, SMALL_THREADS>(h, at);
+}
+
+__global__ void __launch_bounds__(SMALL_THREADS) select_small_kernel(int N, int old, uint32_t need_all,
+                                                                     const float* __restrict__ weights,
+                                                                     int32_t* __restrict__ rows) {
+    __shared__ uint32_t h[HIST_BINS];
+    __shared__ uint32_t s_scan[SMALL_THREADS / WAVE];
+    const int i = SMALL_PER * (int)threadIdx.x;
+    uint32_t key[SMALL_PER], valid = 0;
+#pragma unroll
+    for (int j = 0; j < SMALL_PER; ++j) {
+        key[j] = i + j < old ? weight_key(weights[i + j]) : 0u;
+        valid |= (i + j < old ? 1u : 0u) << j;
+    }
+    uint2 at = make_uint2(0u, need_all);
+    at = small_pass<0>(h, key, valid, at);
+    at = small_pass<1>(h, key, valid, at);
+    at = small_pass<2>(h, key, valid, at);
+    uint32_t above = 0, level = 0;
+#pragma unroll
+    for (int j = 0; j < SMALL_PER; ++j) {
+        const bool v = valid >> j & 1u;
+        above |= ((v ? key[j] > at.x : i + j < N) ? 1u : 0u) << j;
+        level |= (v && key[j] == at.x ? 1u : 0u) << j;
+    }
+    const uint32_t own = (uint32_t)__popc(above) | (uint32_t)__popc(level) << 16;   // each at most SMALL_ROWS in all: 16 bits hold it
+    uint32_t before = wave_scan_u32(own);
+    if ((threadIdx.x & 63) == 63) s_scan[threadIdx.x >> 6] = before;
+    __syncthreads();
+    before -= own;
+    for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) before += s_scan[w];
+    uint32_t pl = before >> 16, out = (before & 0xffffu) + (pl < at.y ? pl : at.y);
+#pragma unroll
+    for (int j = 0; j < SMALL_PER; ++j) {
+        const bool l = level >> j & 1u;
+        if ((above >> j & 1u) || (l && pl < at.y)) rows[out++] = i + j;
+        pl += l ? 1u : 0u;
     }
 }
 
@@ -542,6 +606,11 @@ hipError_t launch_evict_select(int64_t N, const float* weights, int64_t budget, 
         return hipGetLastError();
     }
     const int64_t old = N - recent;
+    if (N <= SMALL_ROWS) {
+        hipLaunchKernelGGL(select_small_kernel, dim3(1), dim3(SMALL_THREADS), 0, st, (int)N, (int)old, (uint32_t)(keep - recent),
+                           weights, rows);
+        return hipGetLastError();
+    }
     SelectState* s = (SelectState*)temp;
     uint2* counts = (uint2*)((char*)temp + align_up(sizeof(SelectState), 256));
     const int64_t all = (N + SELECT_ROWS - 1) / SELECT_ROWS;

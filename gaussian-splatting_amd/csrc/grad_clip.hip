@@ -96,14 +96,14 @@ __device__ __forceinline__ Chunk chunk_of(const NormTable& t, int k, uint32_t ch
     return c;
 }
 template <typename V, typename E>
-__device__ __forceinline__ void for_chunk(const Chunk& c, V vectors, E element) {
+__device__ __forceinline__ void for_chunk(const Chunk& c, int tid, V vectors, E element) {   // tid: 0 .. NORM_THREADS - 1
     const int lo = (c.begin + 15) >> 4, hi = c.end >> 4;
     vectors(lo, hi);
     const int es = type_bytes(c.type);
     if (c.begin != 0 || (c.end & 15) != 0) {   // at most seven elements at either end
         const int head_end = lo << 4 < c.end ? lo << 4 : c.end, tail = hi >= lo ? hi << 4 : c.end;
-        const int x = (int)threadIdx.x < 64 ? c.begin + (int)threadIdx.x * es : tail + ((int)threadIdx.x - 64) * es;
-        if (threadIdx.x < 8 ? x < head_end : threadIdx.x >= 64 && threadIdx.x < 72 && x < c.end) element(x);
+        const int x = tid < 64 ? c.begin + tid * es : tail + (tid - 64) * es;
+        if (tid < 8 ? x < head_end : tid >= 64 && tid < 72 && x < c.end) element(x);
     }
 }
 
@@ -205,6 +205,58 @@ __device__ __forceinline__ uint4 load_vector(const char* p) {
     return __builtin_bit_cast(uint4, ONCE ? __builtin_nontemporal_load(q) : *q);
 }
 
+template <typename S, bool ONCE>
+__device__ __forceinline__ void add_chunk(typename S::T& a, const Chunk& c, int tid) {
+    for_chunk(c, tid, [&](int lo, int hi) {
+        uint4 v[4];
+        if (hi - lo == CHUNK_BYTES / 16) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = load_vector<ONCE>(c.base + 16 * (u * NORM_THREADS + tid));
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = u * NORM_THREADS + tid;
+                v[u] = i >= lo && i < hi ? load_vector<ONCE>(c.base + 16 * i) : make_uint4(0, 0, 0, 0);   // zeros add nothing
+            }
+        }
+        with_type(c.type, [&](auto type) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) add_vector<S, decltype(type)::value>(a, v[u]);
+        });
+    }, [&](int x) {
+        if (c.type == GSO_F32) S::add(a, *(const float*)(c.base + x));
+        else if (c.type == GSO_BF16) S::add(a, bf16_to_float(*(const uint16_t*)(c.base + x)));
+        else S::add(a, f16_to_float(*(const uint16_t*)(c.base + x)));
+    });
+}
+
+// Non-temporal both ways: the scaled gradients are next read by an optimizer that streams six times as much, and keeping
+// them out of the caches leaves there what the norm has put in.
+__device__ __forceinline__ void scale_chunk(const Chunk& c, int tid, float s) {
+    for_chunk(c, tid, [&](int lo, int hi) {
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = u * NORM_THREADS + tid;
+            if (i >= lo && i < hi) v[u] = load_vector<true>(c.base + 16 * i);
+        }
+        with_type(c.type, [&](auto type) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = u * NORM_THREADS + tid;
+                if (i >= lo && i < hi)
+                    __builtin_nontemporal_store(__builtin_bit_cast(f32x4, scale_vector<decltype(type)::value>(v[u], s)),
+                                                reinterpret_cast<f32x4*>(c.base + 16 * i));
+            }
+        });
+    }, [&](int x) {
+        char* p = c.base + x;
+        if (c.type == GSO_F32) *(float*)p = *(const float*)p * s;
+        else if (c.type == GSO_BF16) *(uint16_t*)p = float_to_bf16(bf16_to_float(*(const uint16_t*)p) * s);
+        else *(uint16_t*)p = float_to_f16(f16_to_float(*(const uint16_t*)p) * s);
+    });
+}
+
 // ONCE: the gradients are not read again through the caches' help (a norm alone, or an Adam step, whose other six
 // streams push them out): non-temporal loads, 7.0 TB/s on 1.5 GB where ordinary ones reach 6.2.  A clip reads them
 // again at once; ordinary loads leave up to 256 MB in the last-level cache for it.
@@ -215,28 +267,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_kernel(const NormTable t, u
     int k = find_tensor(t, blockIdx.x);
     for (uint32_t chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
         while (k + 1 < t.n && t.first[k + 1] <= chunk) ++k;
-        const Chunk c = chunk_of(t, k, chunk);
-        for_chunk(c, [&](int lo, int hi) {
-            uint4 v[4];
-            if (hi - lo == CHUNK_BYTES / 16) {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = load_vector<ONCE>(c.base + 16 * (u * NORM_THREADS + (int)threadIdx.x));
-            } else {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int i = u * NORM_THREADS + (int)threadIdx.x;
-                    v[u] = i >= lo && i < hi ? load_vector<ONCE>(c.base + 16 * i) : make_uint4(0, 0, 0, 0);   // zeros add nothing
-                }
-            }
-            with_type(c.type, [&](auto type) {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) add_vector<S, decltype(type)::value>(a, v[u]);
-            });
-        }, [&](int x) {
-            if (c.type == GSO_F32) S::add(a, *(const float*)(c.base + x));
-            else if (c.type == GSO_BF16) S::add(a, bf16_to_float(*(const uint16_t*)(c.base + x)));
-            else S::add(a, f16_to_float(*(const uint16_t*)(c.base + x)));
-        });
+        add_chunk<S, ONCE>(a, chunk_of(t, k, chunk), (int)threadIdx.x);
     }
     a = block_join<S, NORM_THREADS>(a);
     if (threadIdx.x == 0) partial[blockIdx.x] = S::bits(a);
@@ -271,39 +302,66 @@ __global__ void __launch_bounds__(FINISH_THREADS) norm_finish_kernel(const uint6
     }
 }
 
-// Non-temporal both ways: the scaled gradients are next read by an optimizer that streams six times as much, and keeping
-// them out of the caches leaves there what the norm has put in.
-__global__ void __launch_bounds__(NORM_THREADS) scale_kernel(const NormTable t, const NormResult* __restrict__ result) {
-    const float s = result->coefficient;
+// A norm that gso_grad_norm has left in `temp` becomes a coefficient.
+__global__ void coefficient_kernel(NormResult* __restrict__ result, double max_norm, float* __restrict__ norm_out) {
+    result->coefficient = clip_coefficient(result->norm, max_norm);
+    *norm_out = (float)result->norm;
+}
+
+// A few chunks are one workgroup's work, four of them at a time, and one launch's: the norm, and where it is a clip the
+// scaling behind it.
+constexpr int SMALL_THREADS = 4 * NORM_THREADS;
+template <int KIND, bool SCALE>
+__global__ void __launch_bounds__(SMALL_THREADS) norm_small_kernel(const NormTable t, double max_norm,
+                                                                   NormResult* __restrict__ result, float* __restrict__ norm_out) {
+    typedef Share<KIND> S;
+    const int tid = (int)threadIdx.x & (NORM_THREADS - 1);
+    const uint32_t group = (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x / NORM_THREADS);
+    typename S::T a = S::zero();
+    for (uint32_t chunk = group; chunk < t.chunks; chunk += SMALL_THREADS / NORM_THREADS)
+        add_chunk<S, false>(a, chunk_of(t, find_tensor(t, chunk), chunk), tid);
+    const double norm = S::norm(block_join<S, SMALL_THREADS>(a));
+    const float s = clip_coefficient(norm, max_norm);
+    if (threadIdx.x == 0) {
+        result->norm = norm;
+        result->coefficient = s;
+        *norm_out = (float)norm;
+    }
+    if (!SCALE || s == 1.0f) return;
+    for (uint32_t chunk = group; chunk < t.chunks; chunk += SMALL_THREADS / NORM_THREADS)
+        scale_chunk(chunk_of(t, find_tensor(t, chunk), chunk), tid, s);
+}
+
+// Where the consumers of a norm find the coefficient: finished (count = 0), or in at most NORM_THREADS sums, which every
+// workgroup joins for itself; that saves a launch where launches are what counts.
+struct Coefficient {
+    const NormResult* result;
+    const uint64_t* partial;
+    float* norm;
+    double max_norm;
+    int count, kind;
+};
+template <int KIND>
+__device__ __forceinline__ float join_coefficient(const Coefficient& c) {
+    typedef Share<KIND> S;
+    const double norm = S::norm(block_join<S, NORM_THREADS>((int)threadIdx.x < c.count ? S::of(c.partial[threadIdx.x]) : S::zero()));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *c.norm = (float)norm;
+    return clip_coefficient(norm, c.max_norm);
+}
+__device__ __forceinline__ float coefficient_of(const Coefficient& c) {
+    if (c.count == 0) return c.result->coefficient;
+    return c.kind == 2 ? join_coefficient<2>(c) : c.kind == 1 ? join_coefficient<1>(c) : join_coefficient<0>(c);
+}
+
+__global__ void __launch_bounds__(NORM_THREADS) scale_kernel(const NormTable t, const Coefficient coefficient) {
+    const float s = coefficient_of(coefficient);
     if (s == 1.0f) return;   // under the ceiling nothing changes, and nothing is read
-    const Chunk c = chunk_of(t, find_tensor(t, blockIdx.x), blockIdx.x);
-    for_chunk(c, [&](int lo, int hi) {
-        uint4 v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = u * NORM_THREADS + (int)threadIdx.x;
-            if (i >= lo && i < hi) v[u] = load_vector<true>(c.base + 16 * i);
-        }
-        with_type(c.type, [&](auto type) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int i = u * NORM_THREADS + (int)threadIdx.x;
-                if (i >= lo && i < hi)
-                    __builtin_nontemporal_store(__builtin_bit_cast(f32x4, scale_vector<decltype(type)::value>(v[u], s)),
-                                                reinterpret_cast<f32x4*>(c.base + 16 * i));
-            }
-        });
-    }, [&](int x) {
-        char* p = c.base + x;
-        if (c.type == GSO_F32) *(float*)p = *(const float*)p * s;
-        else if (c.type == GSO_BF16) *(uint16_t*)p = float_to_bf16(bf16_to_float(*(const uint16_t*)p) * s);
-        else *(uint16_t*)p = float_to_f16(f16_to_float(*(const uint16_t*)p) * s);
-    });
+    scale_chunk(chunk_of(t, find_tensor(t, blockIdx.x), blockIdx.x), (int)threadIdx.x, s);
 }
 
 // Two vectors of each stream a thread, all loads first, non-temporal: every value is used once in a step.
-__global__ void __launch_bounds__(NORM_THREADS) adam_clipped_kernel(const AdamTable t, const NormResult* __restrict__ result) {
-    const float s = result->coefficient;
+__global__ void __launch_bounds__(NORM_THREADS) adam_clipped_kernel(const AdamTable t, const Coefficient coefficient) {
+    const float s = coefficient_of(coefficient);
     const int k = find_tensor(t, blockIdx.x);
     const AdamEntry& e = t.e[k];
     const int64_t base = (int64_t)(blockIdx.x - t.first[k]) * ADAM_CHUNK;
@@ -354,10 +412,10 @@ __global__ void __launch_bounds__(NORM_THREADS) adam_clipped_kernel(const AdamTa
 // of the listed rows only, four each in flight.  The list's order is that of arrival; every element is updated on
 // its own, so nothing depends on it.
 __global__ void __launch_bounds__(NORM_THREADS) adam_clipped_sparse_kernel(const AdamTable t, const uint8_t* __restrict__ visible,
-                                                                           const NormResult* __restrict__ result) {
+                                                                           const Coefficient coefficient) {
     __shared__ uint16_t s_row[SPARSE_CHUNK];
     __shared__ uint32_t s_count;
-    const float s = result->coefficient;
+    const float s = coefficient_of(coefficient);
     const int k = find_tensor(t, blockIdx.x);
     const AdamEntry& e = t.e[k];
     const uint32_t W = e.width, R = W < SPARSE_CHUNK ? SPARSE_CHUNK / W : 1;
@@ -439,9 +497,10 @@ size_t norm_temp_bytes(int n) {
 
 static uint64_t* norm_partials(void* temp) { return (uint64_t*)((char*)temp + 256); }
 
-// Calls launch(table) for every group of tensors that fits a table.
+// Calls launch(table, whether it is the only one) for every group of tensors that fits a table.
 template <typename F>
 static hipError_t for_each_table(int n, const void* const* ptrs, const int64_t* numels, const int* types, F launch) {
+    bool first = true;
     for (int i = 0; i < n;) {
         NormTable t;
         t.n = 0;
@@ -456,7 +515,8 @@ static hipError_t for_each_table(int n, const void* const* ptrs, const int64_t* 
             ++t.n;
         }
         if (t.n == 0) break;
-        launch(t);
+        launch(t, first && i == n);
+        first = false;
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -469,44 +529,89 @@ static void launch_norm(const NormTable& t, bool read_again, unsigned groups, ui
     else hipLaunchKernelGGL((norm_kernel<KIND, true>), dim3(groups), dim3(NORM_THREADS), 0, st, t, p);
 }
 
-hipError_t launch_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int kind,
-                            bool read_again, void* temp, int* partials, hipStream_t st) {
-    int count = 0;
-    const hipError_t e = for_each_table(n, grads, numels, types, [&](const NormTable& t) {
+template <int KIND>
+static void launch_small(const NormTable& t, bool scale, double max_norm, NormResult* r, float* norm, hipStream_t st) {
+    if (scale) hipLaunchKernelGGL((norm_small_kernel<KIND, true>), dim3(1), dim3(SMALL_THREADS), 0, st, t, max_norm, r, norm);
+    else hipLaunchKernelGGL((norm_small_kernel<KIND, false>), dim3(1), dim3(SMALL_THREADS), 0, st, t, max_norm, r, norm);
+}
+
+template <int KIND>
+static void launch_finish(const uint64_t* p, int count, double max_norm, NormResult* r, float* norm, hipStream_t st) {
+    hipLaunchKernelGGL(norm_finish_kernel<KIND>, dim3(1), dim3(FINISH_THREADS), 0, st, p, count, max_norm, r, norm);
+}
+
+// The norm of the gradients for whoever reads it next.  FINISH: the result in the temp area and in *norm; otherwise
+// *c says where the coefficient is found.  A clip of a few chunks is done at once (*scaled).
+constexpr uint32_t SMALL_CHUNKS = 16;
+enum NormUse { NORM_ONLY, NORM_CLIP, NORM_STEP };
+static hipError_t launch_norm_for(NormUse use, int n, const void* const* grads, const int64_t* numels, const int* types,
+                                  int kind, double max_norm, void* temp, float* norm, hipStream_t st, Coefficient* c,
+                                  bool* scaled) {
+    NormResult* r = (NormResult*)temp;
+    int count = 0, small = 0;
+    hipError_t e = for_each_table(n, grads, numels, types, [&](const NormTable& t, bool alone) {
+        if (alone && t.chunks <= SMALL_CHUNKS) {
+            small = 1;
+            if (kind == 2) launch_small<2>(t, use == NORM_CLIP, max_norm, r, norm, st);
+            else if (kind == 1) launch_small<1>(t, use == NORM_CLIP, max_norm, r, norm, st);
+            else launch_small<0>(t, use == NORM_CLIP, max_norm, r, norm, st);
+            return;
+        }
         const uint32_t rounds = (t.chunks + NORM_GROUPS - 1) / NORM_GROUPS;   // the same number for every workgroup
         const unsigned groups = (t.chunks + rounds - 1) / rounds;
         uint64_t* p = norm_partials(temp) + count;
-        if (kind == 2) launch_norm<2>(t, read_again, groups, p, st);
-        else if (kind == 1) launch_norm<1>(t, read_again, groups, p, st);
-        else launch_norm<0>(t, read_again, groups, p, st);
+        if (kind == 2) launch_norm<2>(t, use == NORM_CLIP, groups, p, st);
+        else if (kind == 1) launch_norm<1>(t, use == NORM_CLIP, groups, p, st);
+        else launch_norm<0>(t, use == NORM_CLIP, groups, p, st);
         count += (int)groups;
     });
-    *partials = count;
+    if (e != hipSuccess) return e;
+    *scaled = small && use == NORM_CLIP;
+    const bool join_later = use != NORM_ONLY && count > 0 && count <= NORM_THREADS;
+    if (!small && !join_later) {
+        if (kind == 2) launch_finish<2>(norm_partials(temp), count, max_norm, r, norm, st);
+        else if (kind == 1) launch_finish<1>(norm_partials(temp), count, max_norm, r, norm, st);
+        else launch_finish<0>(norm_partials(temp), count, max_norm, r, norm, st);
+        e = hipGetLastError();
+    }
+    *c = {r, norm_partials(temp), norm, max_norm, join_later ? count : 0, kind};
     return e;
 }
 
-hipError_t launch_norm_finish(void* temp, int partials, int kind, double max_norm, float* norm, hipStream_t st) {
-    NormResult* r = (NormResult*)temp;
-    const uint64_t* p = norm_partials(temp);
-    const dim3 grid(1), block(FINISH_THREADS);
-    if (kind == 2) hipLaunchKernelGGL(norm_finish_kernel<2>, grid, block, 0, st, p, partials, max_norm, r, norm);
-    else if (kind == 1) hipLaunchKernelGGL(norm_finish_kernel<1>, grid, block, 0, st, p, partials, max_norm, r, norm);
-    else hipLaunchKernelGGL(norm_finish_kernel<0>, grid, block, 0, st, p, partials, max_norm, r, norm);
+// The same where gso_grad_norm has been called for these gradients and this temp area.
+static hipError_t launch_coefficient(int kind, double max_norm, void* temp, float* norm, hipStream_t st, Coefficient* c) {
+    hipLaunchKernelGGL(coefficient_kernel, dim3(1), dim3(1), 0, st, (NormResult*)temp, max_norm, norm);
+    *c = {(NormResult*)temp, norm_partials(temp), norm, max_norm, 0, kind};
     return hipGetLastError();
 }
 
+hipError_t launch_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int kind, void* temp,
+                            float* norm, hipStream_t st) {
+    Coefficient c;
+    bool scaled;
+    return launch_norm_for(NORM_ONLY, n, grads, numels, types, kind, 0.0, temp, norm, st, &c, &scaled);
+}
+
 hipError_t launch_clip_grads(int n, void* const* grads, const int64_t* numels, const int* types, int kind, double max_norm,
-                             void* temp, int partials, float* norm, hipStream_t st) {
-    const hipError_t e = launch_norm_finish(temp, partials, kind, max_norm, norm, st);
-    if (e != hipSuccess) return e;
-    return for_each_table(n, (const void* const*)grads, numels, types, [&](const NormTable& t) {
-        hipLaunchKernelGGL(scale_kernel, dim3(t.chunks), dim3(NORM_THREADS), 0, st, t, (const NormResult*)temp);
+                             bool norm_known, void* temp, float* norm, hipStream_t st) {
+    Coefficient c;
+    bool scaled = false;
+    const void* const* g = (const void* const*)grads;
+    const hipError_t e = norm_known ? launch_coefficient(kind, max_norm, temp, norm, st, &c)
+                                    : launch_norm_for(NORM_CLIP, n, g, numels, types, kind, max_norm, temp, norm, st, &c, &scaled);
+    if (e != hipSuccess || scaled) return e;
+    return for_each_table(n, g, numels, types, [&](const NormTable& t, bool) {
+        hipLaunchKernelGGL(scale_kernel, dim3(t.chunks), dim3(NORM_THREADS), 0, st, t, c);
     });
 }
 
-hipError_t launch_adam_clipped(int n, const GsoAdamTensor* tensors, const uint8_t* visible, int kind, double max_norm,
-                               void* temp, int partials, float* norm, hipStream_t st) {
-    hipError_t e = launch_norm_finish(temp, partials, kind, max_norm, norm, st);
+hipError_t launch_adam_clipped(int ngrads, const void* const* grads, const int64_t* numels, const int* types, int n,
+                               const GsoAdamTensor* tensors, const uint8_t* visible, int kind, double max_norm,
+                               bool norm_known, void* temp, float* norm, hipStream_t st) {
+    Coefficient c;
+    bool scaled;
+    hipError_t e = norm_known ? launch_coefficient(kind, max_norm, temp, norm, st, &c)
+                              : launch_norm_for(NORM_STEP, ngrads, grads, numels, types, kind, max_norm, temp, norm, st, &c, &scaled);
     for (int i = 0; i < n && e == hipSuccess;) {
         AdamTable t;
         t.n = 0;
@@ -525,8 +630,8 @@ hipError_t launch_adam_clipped(int n, const GsoAdamTensor* tensors, const uint8_
         }
         if (t.n == 0) break;
         const dim3 grid((unsigned)groups), block(NORM_THREADS);
-        if (visible) hipLaunchKernelGGL(adam_clipped_sparse_kernel, grid, block, 0, st, t, visible, (const NormResult*)temp);
-        else hipLaunchKernelGGL(adam_clipped_kernel, grid, block, 0, st, t, (const NormResult*)temp);
+        if (visible) hipLaunchKernelGGL(adam_clipped_sparse_kernel, grid, block, 0, st, t, visible, c);
+        else hipLaunchKernelGGL(adam_clipped_kernel, grid, block, 0, st, t, c);
         e = hipGetLastError();
     }
     return e;

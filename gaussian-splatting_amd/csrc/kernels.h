@@ -214,13 +214,13 @@ hipError_t launch_gather_rows(const void* src, void* dst, const uint32_t* src_of
 // Gradient norm, clipping and the Adam step under a ceiling (grad_clip.hip); kind: 0 max |g|, 1 sum |g|, 2 sqrt(sum g^2).
 bool norm_fits(int n, const int64_t* numels);
 size_t norm_temp_bytes(int n);
-hipError_t launch_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int kind,
-                            bool read_again, void* temp, int* partials, hipStream_t st);
-hipError_t launch_norm_finish(void* temp, int partials, int kind, double max_norm, float* norm, hipStream_t st);
+hipError_t launch_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int kind, void* temp,
+                            float* norm, hipStream_t st);
 hipError_t launch_clip_grads(int n, void* const* grads, const int64_t* numels, const int* types, int kind, double max_norm,
-                             void* temp, int partials, float* norm, hipStream_t st);
-hipError_t launch_adam_clipped(int n, const GsoAdamTensor* tensors, const uint8_t* visible, int kind, double max_norm,
-                               void* temp, int partials, float* norm, hipStream_t st);
+                             bool norm_known, void* temp, float* norm, hipStream_t st);
+hipError_t launch_adam_clipped(int ngrads, const void* const* grads, const int64_t* numels, const int* types, int n,
+                               const GsoAdamTensor* tensors, const uint8_t* visible, int kind, double max_norm,
+                               bool norm_known, void* temp, float* norm, hipStream_t st);
 // Accumulated weights and eviction (evict.hip).
 hipError_t launch_accumulate_weights(int64_t N, float* weights, int views, const float* const* contributions,
                                      const float* opacity, float decay, hipStream_t st);

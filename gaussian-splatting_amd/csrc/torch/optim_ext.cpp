@@ -108,26 +108,24 @@ void check_may_wait(const char* what) {
 
 struct Norm {
     Tensor temp, value;
-    int partials = 0;
+    size_t bytes;
+    explicit Norm(const Grads& g) : bytes(gso_norm_temp_bytes(g.n())) {
+        const auto opt = torch::TensorOptions().device(g.own[0].device());
+        temp = torch::empty({(int64_t)bytes}, opt.dtype(torch::kUInt8));
+        value = torch::empty({}, opt.dtype(torch::kFloat32));
+    }
+    float* out() const { return value.data_ptr<float>(); }
+    void form(const Grads& g, int kind, void* st, const char* what) {
+        check_rc(gso_grad_norm(g.n(), g.cptr(), g.numel.data(), g.type.data(), kind, temp.data_ptr(), bytes, out(), st), what);
+    }
+    // error_if_nonfinite: the norm before anything changes
+    void look(const Grads& g, int kind, void* st, const char* what) {
+        form(g, kind, st, what);
+        const float norm = value.item<float>();
+        TORCH_CHECK(std::isfinite(norm), what, ": the total norm of the gradients is ", norm,
+                    " (error_if_nonfinite); nothing was changed");
+    }
 };
-
-Norm sums_of(const Grads& g, int kind, bool read_again, void* st, const char* what) {
-    Norm r;
-    const auto opt = torch::TensorOptions().device(g.own[0].device());
-    const size_t bytes = gso_norm_temp_bytes(g.n());
-    r.temp = torch::empty({(int64_t)bytes}, opt.dtype(torch::kUInt8));
-    r.value = torch::empty({}, opt.dtype(torch::kFloat32));
-    check_rc(gso_grad_norm(g.n(), g.cptr(), g.numel.data(), g.type.data(), kind, read_again, r.temp.data_ptr(), bytes,
-                           &r.partials, st),
-             what);
-    return r;
-}
-
-void raise_if_nonfinite(Norm& r, int kind, void* st, const char* what) {
-    check_rc(gso_norm_finish(r.temp.data_ptr(), r.partials, kind, r.value.data_ptr<float>(), st), what);
-    TORCH_CHECK(std::isfinite(r.value.item<float>()), what, ": the total norm of the gradients is ", r.value.item<float>(),
-                " (error_if_nonfinite); nothing was changed");
-}
 
 Tensor grad_norm(const std::vector<Tensor>& params, double norm_type) {
     const char* what = "grad_norm";
@@ -135,9 +133,8 @@ Tensor grad_norm(const std::vector<Tensor>& params, double norm_type) {
     const Grads g = collect(params, what);
     if (g.own.empty()) return torch::zeros({});
     c10::DeviceGuard guard(g.own[0].device());
-    void* st = stream_on(g.own[0].device());
-    Norm r = sums_of(g, kind, false, st, what);
-    check_rc(gso_norm_finish(r.temp.data_ptr(), r.partials, kind, r.value.data_ptr<float>(), st), what);
+    Norm r(g);
+    r.form(g, kind, stream_on(g.own[0].device()), what);
     return r.value;
 }
 
@@ -151,10 +148,10 @@ Tensor clip_grad_norm(const std::vector<Tensor>& params, double max_norm, double
     c10::DeviceGuard guard(g.own[0].device());
     if (error_if_nonfinite) check_may_wait(what);
     void* st = stream_on(g.own[0].device());
-    Norm r = sums_of(g, kind, true, st, what);
-    if (error_if_nonfinite) raise_if_nonfinite(r, kind, st, what);
-    check_rc(gso_clip_grads(g.n(), g.ptr.data(), g.numel.data(), g.type.data(), kind, max_norm, r.temp.data_ptr(), r.partials,
-                            r.value.data_ptr<float>(), st),
+    Norm r(g);
+    if (error_if_nonfinite) r.look(g, kind, st, what);
+    check_rc(gso_clip_grads(g.n(), g.ptr.data(), g.numel.data(), g.type.data(), kind, max_norm, error_if_nonfinite,
+                            r.temp.data_ptr(), r.bytes, r.out(), st),
              what);
     torch::NoGradGuard no_grad;
     for (size_t i = 0; i < g.own.size(); ++i) {
@@ -227,10 +224,11 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
         table.push_back(a);
     }
     void* st = stream_on(dev);
-    Norm r = sums_of(g, kind, false, st, what);
-    if (error_if_nonfinite) raise_if_nonfinite(r, kind, st, what);
-    check_rc(gso_adam_clipped((int)table.size(), table.data(), visible.defined() ? (const uint8_t*)visible.data_ptr() : nullptr,
-                              kind, max_norm, r.temp.data_ptr(), r.partials, r.value.data_ptr<float>(), st),
+    Norm r(g);
+    if (error_if_nonfinite) r.look(g, kind, st, what);
+    check_rc(gso_adam_clipped(g.n(), g.cptr(), g.numel.data(), g.type.data(), (int)table.size(), table.data(),
+                              visible.defined() ? (const uint8_t*)visible.data_ptr() : nullptr, kind, max_norm,
+                              error_if_nonfinite, r.temp.data_ptr(), r.bytes, r.out(), st),
              what);
     for (size_t i : counted) {
         if (on_host(steps[i])) *steps[i].data_ptr<float>() += 1.0f;

@@ -454,17 +454,17 @@ int gso_gather_rows(const void* src, void* dst, const uint32_t* src_of_dst, int6
  *   norm = sqrt(sum g^2) (norm_type 2), sum |g| (1) or max |g| (0) over all elements of all tensors; a NaN anywhere
  *          makes it NaN.  Sums are held in 64 bits and added in a fixed order: the same bits in every run.
  *   c    = min(1, max_norm / (norm + 1e-6)), formed in 64 bits from the unrounded norm, rounded once to float32
- * `grads` are HOST arrays of n device pointers with their element counts and types (GsoType); elements are contiguous,
- * pointers aligned to an element, a count of zero (pointer ignored) is allowed.  Tensors may be of different types.
- *   gso_grad_norm: sums into `temp` (device, 8-byte aligned, gso_norm_temp_bytes(n) bytes), *partials =
- *     how many sums it left there.  read_again: nonzero when gso_clip_grads follows (the loads then leave what fits in
- *     the caches).
- *   gso_norm_finish: *norm (device, float32) from `temp`.
- *   gso_clip_grads: the same, then g <- g * c in place, each product rounded once to the tensor's type; with c = 1
- *     nothing is read or written.  No two tensors may share memory.
- *   gso_adam_clipped: *norm, then Adam's update of every tensor with the gradient c * g (the product rounded to float32,
- *     as clipping in place would store it; the gradients keep their values), operation by operation gso_adam_update's.
- *     `visible`: device bytes, one per row, or NULL; applies to every tensor of the call.
+ * `grads`, `numels`, `types`: HOST arrays of n device pointers, aligned to an element, of element counts (zero is
+ * allowed, the pointer is then ignored) and of GsoTypes; a tensor's elements are contiguous, tensors may be of different
+ * types.  `temp`: device, 8-byte aligned, gso_norm_temp_bytes(n) bytes.
+ *   gso_grad_norm: *norm (device, float32); also left in `temp`.
+ *   gso_clip_grads: *norm, then g <- g * c in place, each product rounded once to the tensor's type; with c = 1
+ *     nothing is written.  No two tensors may share memory.
+ *   gso_adam_clipped: *norm of the `ngrads` gradients, then Adam's update of the `n` tensors with the gradient c * g (the
+ *     product rounded to float32, as clipping in place would store it; the gradients keep their values), operation by
+ *     operation gso_adam_update's.  `visible`: device bytes, one per row, or NULL; applies to every tensor.
+ *   norm_known: nonzero when gso_grad_norm was called for the same gradients with this `temp` and they have not changed
+ *     (a caller that looked at the norm first); it is not formed again then.
  * No call waits for the device, and all can be captured into a graph (the bias corrections are then frozen). */
 typedef enum { GSO_F32 = 0, GSO_BF16 = 1, GSO_F16 = 2 } GsoType;
 typedef struct {
@@ -477,13 +477,13 @@ typedef struct {
     double lr, beta1, beta2, eps, bias_correction1, bias_correction2_sqrt;   /* as gso_adam_update takes them */
 } GsoAdamTensor;
 size_t gso_norm_temp_bytes(int n);
-int gso_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type, int read_again,
-                  void* temp, size_t temp_bytes, int* partials, void* stream);
-int gso_norm_finish(void* temp, int partials, int norm_type, float* norm, void* stream);
+int gso_grad_norm(int n, const void* const* grads, const int64_t* numels, const int* types, int norm_type, void* temp,
+                  size_t temp_bytes, float* norm, void* stream);
 int gso_clip_grads(int n, void* const* grads, const int64_t* numels, const int* types, int norm_type, double max_norm,
-                   void* temp, int partials, float* norm, void* stream);
-int gso_adam_clipped(int n, const GsoAdamTensor* tensors, const uint8_t* visible, int norm_type, double max_norm,
-                     void* temp, int partials, float* norm, void* stream);
+                   int norm_known, void* temp, size_t temp_bytes, float* norm, void* stream);
+int gso_adam_clipped(int ngrads, const void* const* grads, const int64_t* numels, const int* types, int n,
+                     const GsoAdamTensor* tensors, const uint8_t* visible, int norm_type, double max_norm, int norm_known,
+                     void* temp, size_t temp_bytes, float* norm, void* stream);
 
 /* A model within a row budget: the views' blending weights are accumulated per Gaussian, and the lightest rows go.
  * No counterpart in the reference, whose model only shrinks by opacity and size (scene/gaussian_model.py:237-247).

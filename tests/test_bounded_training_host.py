@@ -65,38 +65,34 @@ def test_c_abi_refuses_bad_arguments():
     L = lib()
     ARG, OVERFLOW, BUFFER = -1, -3, -4
     one, big = (C.c_int64 * 1)(10), (C.c_int64 * 1)(1 << 50)
-    neg, zero = (C.c_int64 * 1)(-1), (C.c_int64 * 1)(0)
+    neg = (C.c_int64 * 1)(-1)
     t0, t9 = (C.c_int * 1)(0), (C.c_int * 1)(9)
     good, odd, null = (C.c_void_p * 1)(4096), (C.c_void_p * 1)(4097), (C.c_void_p * 1)(None)
-    cnt = C.c_int(0)
     size = L.gso_norm_temp_bytes(1)
     assert size > 0 and L.gso_norm_temp_bytes(-1) == 0 and L.gso_norm_temp_bytes(0) > 0
 
-    def norm(n=1, g=good, k=one, t=t0, kind=2, temp=4096, bytes_=size, out=C.byref(cnt)):
-        return L.gso_grad_norm(n, g, k, t, kind, 0, temp, bytes_, out, None)
+    def norm(n=1, g=good, k=one, t=t0, kind=2, temp=4096, bytes_=size, out=4096):
+        return L.gso_grad_norm(n, g, k, t, kind, temp, bytes_, out, None)
     assert norm(n=-1) == ARG and norm(g=null) == ARG and norm(g=odd) == ARG and norm(k=neg) == ARG and norm(t=t9) == ARG
     assert norm(kind=3) == ARG and norm(kind=-1) == ARG and norm(temp=None) == ARG and norm(temp=4100) == ARG
     assert norm(out=None) == ARG and norm(g=None) == ARG and norm(bytes_=8) == BUFFER
-    assert norm(k=big, bytes_=1 << 60) == OVERFLOW
-    assert norm(g=null, k=zero) == 0 and cnt.value == 0          # nothing to read: nothing is launched
-    assert norm(n=0, g=None, k=None, t=None) == 0
-    assert L.gso_norm_finish(None, 0, 2, 4096, None) == ARG and L.gso_norm_finish(4096, 0, 2, None, None) == ARG
-    assert L.gso_norm_finish(4096, -1, 2, 4096, None) == ARG and L.gso_norm_finish(4096, 0, 7, 4096, None) == ARG
+    assert norm(k=big) == OVERFLOW
 
-    def clip(max_norm=1.0, g=good, norm_out=4096, n=1):
-        return L.gso_clip_grads(n, g, one, t0, 2, max_norm, 4096, 1, norm_out, None)
-    assert clip(-1.0) == ARG and clip(math.nan) == ARG and clip(g=odd) == ARG and clip(norm_out=None) == ARG and clip(n=-1) == ARG
+    def clip(max_norm=1.0, g=good, out=4096, n=1, bytes_=size):
+        return L.gso_clip_grads(n, g, one, t0, 2, max_norm, 0, 4096, bytes_, out, None)
+    assert clip(-1.0) == ARG and clip(math.nan) == ARG and clip(g=odd) == ARG and clip(out=None) == ARG and clip(n=-1) == ARG
+    assert clip(bytes_=size - 1) == BUFFER
 
     class Adam(C.Structure):
         _fields_ = [(n, C.c_void_p) for n in ("param", "grad", "m", "v")] + [("rows", C.c_int64), ("width", C.c_int64)] + \
                    [(n, C.c_double) for n in ("lr", "b1", "b2", "eps", "bc1", "bc2")]
 
-    def adam(max_norm=1.0, n=1, **kw):
+    def adam(max_norm=1.0, n=1, out=4096, **kw):
         f = dict(param=4096, grad=4096, m=4096, v=4096, rows=10, width=3, lr=0.1, b1=0.9, b2=0.99, eps=1e-8, bc1=1.0, bc2=1.0)
         f.update(kw)
-        return L.gso_adam_clipped(n, C.byref(Adam(**f)), None, 2, max_norm, 4096, 1, 4096, None)
+        return L.gso_adam_clipped(1, good, one, t0, n, C.byref(Adam(**f)), None, 2, max_norm, 0, 4096, size, out, None)
     assert adam(-1.0) == ARG and adam(n=-1) == ARG and adam(param=None) == ARG and adam(grad=4097) == ARG
-    assert adam(rows=-1) == ARG and adam(width=0) == ARG and adam(bc1=0.0) == ARG and adam(bc2=math.nan) == ARG
+    assert adam(rows=-1) == ARG and adam(width=0) == ARG and adam(bc1=0.0) == ARG and adam(bc2=math.nan) == ARG and adam(out=None) == ARG
     assert adam(rows=1 << 31) == OVERFLOW and adam(rows=1 << 30, width=1 << 12) == OVERFLOW
 
     assert L.gso_accumulate_weights(-1, 4096, 0, None, None, 1.0, None) == ARG

@@ -104,7 +104,7 @@ def _weights(kind, N, gen):
 
 
 @pytest.mark.parametrize("kind", ["random", "equal", "zeros", "few_values", "near", "special"])
-@pytest.mark.parametrize("N", [1, 2, 63, 256, 1000, 4095, 4096, 4097, 70001])
+@pytest.mark.parametrize("N", [1, 2, 63, 256, 1000, 4095, 4096, 4097, 8191, 8192, 8193, 70001])
 def test_selection(kind, N):
     import gsplat_optim as G
     gen = torch.Generator(device="cuda").manual_seed(N)
