@@ -264,9 +264,19 @@ template <int KIND, bool ONCE>
 __global__ void __launch_bounds__(NORM_THREADS) norm_kernel(const NormTable t, uint64_t* __restrict__ partial) {
     typedef Share<KIND> S;
     typename S::T a = S::zero();
-    int k = find_tensor(t, blockIdx.x);
+    // The first chunks of all tensors, one a lane: a chunk's tensor is then found with a few ballots, where a walk through
+    // the kernel's arguments in memory costs a round of loads for every chunk.
+    constexpr int HELD = (NORM_TABLE + WAVE - 1) / WAVE;
+    uint32_t first[HELD];
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+        const int i = j * WAVE + (int)(threadIdx.x & (WAVE - 1));
+        first[j] = i < t.n ? t.first[i] : 0xffffffffu;
+    }
     for (uint32_t chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
-        while (k + 1 < t.n && t.first[k + 1] <= chunk) ++k;
+        int k = -1;
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) k += __popcll(__ballot(first[j] <= chunk));
         add_chunk<S, ONCE>(a, chunk_of(t, k, chunk), (int)threadIdx.x);
     }
     a = block_join<S, NORM_THREADS>(a);
