@@ -140,16 +140,22 @@ struct Share<0> {
     static __device__ __forceinline__ double norm(T a) { return (double)__builtin_bit_cast(float, a); }
 };
 
-// The workgroup's threads joined in a fixed order; the result is valid in every thread.
-template <typename S, int THREADS>
-__device__ __forceinline__ typename S::T block_join(typename S::T v) {
-    __shared__ uint64_t s_w[THREADS / WAVE];
+template <typename S>
+__device__ __forceinline__ typename S::T wave_join(typename S::T v) {
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
         const uint64_t b = S::bits(v);
         const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)b, d, WAVE), hi = (uint32_t)__shfl_xor((int)(uint32_t)(b >> 32), d, WAVE);
         v = S::join(v, S::of((uint64_t)hi << 32 | lo));
     }
+    return v;
+}
+
+// The workgroup's threads joined in a fixed order; the result is valid in every thread.
+template <typename S, int THREADS>
+__device__ __forceinline__ typename S::T block_join(typename S::T v) {
+    __shared__ uint64_t s_w[THREADS / WAVE];
+    v = wave_join<S>(v);
     if ((threadIdx.x & (WAVE - 1)) == 0) s_w[threadIdx.x / WAVE] = S::bits(v);
     __syncthreads();
     v = S::of(s_w[0]);
@@ -342,8 +348,9 @@ __global__ void __launch_bounds__(SMALL_THREADS) norm_small_kernel(const NormTab
         scale_chunk(chunk_of(t, find_tensor(t, chunk), chunk), tid, s);
 }
 
-// Where the consumers of a norm find the coefficient: finished (count = 0), or in at most NORM_THREADS sums, which every
-// workgroup joins for itself; that saves a launch where launches are what counts.
+// Where the consumers of a norm find the coefficient: finished (count = 0), or in at most NORM_GROUPS sums, which every
+// workgroup joins for itself in the order of norm_finish_kernel; that saves a launch where the consumer has few
+// workgroups.
 struct Coefficient {
     const NormResult* result;
     const uint64_t* partial;
@@ -351,10 +358,33 @@ struct Coefficient {
     double max_norm;
     int count, kind;
 };
+static_assert(NORM_GROUPS <= 2 * FINISH_THREADS, "two sums a thread of norm_finish_kernel");
 template <int KIND>
 __device__ __forceinline__ float join_coefficient(const Coefficient& c) {
     typedef Share<KIND> S;
-    const double norm = S::norm(block_join<S, NORM_THREADS>((int)threadIdx.x < c.count ? S::of(c.partial[threadIdx.x]) : S::zero()));
+    constexpr int PARTS = FINISH_THREADS / NORM_THREADS;   // threads of the other kernel that a thread stands for
+    __shared__ uint64_t s_w[FINISH_THREADS / WAVE];
+    typename S::T v[PARTS];
+#pragma unroll
+    for (int j = 0; j < PARTS; ++j) {
+        const int i = (int)threadIdx.x + j * NORM_THREADS;
+        v[j] = S::join(i < c.count ? S::of(c.partial[i]) : S::zero(),
+                       i + FINISH_THREADS < c.count ? S::of(c.partial[i + FINISH_THREADS]) : S::zero());
+    }
+#pragma unroll
+    for (int j = 0; j < PARTS; ++j) {
+        if (j * NORM_THREADS >= c.count) {   // nothing from here on
+            if ((threadIdx.x & (WAVE - 1)) == 0) s_w[threadIdx.x / WAVE + j * (NORM_THREADS / WAVE)] = S::bits(S::zero());
+            continue;
+        }
+        const typename S::T w = wave_join<S>(v[j]);
+        if ((threadIdx.x & (WAVE - 1)) == 0) s_w[threadIdx.x / WAVE + j * (NORM_THREADS / WAVE)] = S::bits(w);
+    }
+    __syncthreads();
+    typename S::T a = S::of(s_w[0]);
+#pragma unroll
+    for (int w = 1; w < FINISH_THREADS / WAVE; ++w) a = S::join(a, S::of(s_w[w]));
+    const double norm = S::norm(a);
     if (blockIdx.x == 0 && threadIdx.x == 0) *c.norm = (float)norm;
     return clip_coefficient(norm, c.max_norm);
 }
@@ -551,12 +581,14 @@ static void launch_finish(const uint64_t* p, int count, double max_norm, NormRes
 }
 
 // The norm of the gradients for whoever reads it next.  FINISH: the result in the temp area and in *norm; otherwise
-// *c says where the coefficient is found.  A clip of a few chunks is done at once (*scaled).
+// *c says where the coefficient is found.  A clip of a few chunks is done at once (*scaled).  `consumers`: workgroups of
+// what reads the coefficient.
 constexpr uint32_t SMALL_CHUNKS = 16;
+constexpr int64_t JOIN_CONSUMERS = 1024;   // clip of 10 MB: 9.5 us with, 11.2 without; of 25 MB (1539): 16.9 and 15.5
 enum NormUse { NORM_ONLY, NORM_CLIP, NORM_STEP };
 static hipError_t launch_norm_for(NormUse use, int n, const void* const* grads, const int64_t* numels, const int* types,
-                                  int kind, double max_norm, void* temp, float* norm, hipStream_t st, Coefficient* c,
-                                  bool* scaled) {
+                                  int kind, double max_norm, int64_t consumers, void* temp, float* norm, hipStream_t st,
+                                  Coefficient* c, bool* scaled) {
     NormResult* r = (NormResult*)temp;
     int count = 0, small = 0;
     hipError_t e = for_each_table(n, grads, numels, types, [&](const NormTable& t, bool alone) {
@@ -577,7 +609,7 @@ static hipError_t launch_norm_for(NormUse use, int n, const void* const* grads, 
     });
     if (e != hipSuccess) return e;
     *scaled = small && use == NORM_CLIP;
-    const bool join_later = use != NORM_ONLY && count > 0 && count <= NORM_THREADS;
+    const bool join_later = use != NORM_ONLY && count > 0 && count <= NORM_GROUPS && consumers <= JOIN_CONSUMERS;
     if (!small && !join_later) {
         if (kind == 2) launch_finish<2>(norm_partials(temp), count, max_norm, r, norm, st);
         else if (kind == 1) launch_finish<1>(norm_partials(temp), count, max_norm, r, norm, st);
@@ -599,7 +631,7 @@ hipError_t launch_grad_norm(int n, const void* const* grads, const int64_t* nume
                             float* norm, hipStream_t st) {
     Coefficient c;
     bool scaled;
-    return launch_norm_for(NORM_ONLY, n, grads, numels, types, kind, 0.0, temp, norm, st, &c, &scaled);
+    return launch_norm_for(NORM_ONLY, n, grads, numels, types, kind, 0.0, 0, temp, norm, st, &c, &scaled);
 }
 
 hipError_t launch_clip_grads(int n, void* const* grads, const int64_t* numels, const int* types, int kind, double max_norm,
@@ -607,12 +639,21 @@ hipError_t launch_clip_grads(int n, void* const* grads, const int64_t* numels, c
     Coefficient c;
     bool scaled = false;
     const void* const* g = (const void* const*)grads;
+    int64_t chunks = 0;
+    for (int i = 0; i < n; ++i) chunks += chunks_of(g[i], numels[i], types[i]);
     const hipError_t e = norm_known ? launch_coefficient(kind, max_norm, temp, norm, st, &c)
-                                    : launch_norm_for(NORM_CLIP, n, g, numels, types, kind, max_norm, temp, norm, st, &c, &scaled);
+                                    : launch_norm_for(NORM_CLIP, n, g, numels, types, kind, max_norm, chunks, temp, norm, st, &c,
+                                                      &scaled);
     if (e != hipSuccess || scaled) return e;
     return for_each_table(n, g, numels, types, [&](const NormTable& t, bool) {
         hipLaunchKernelGGL(scale_kernel, dim3(t.chunks), dim3(NORM_THREADS), 0, st, t, c);
     });
+}
+
+// Workgroups of a tensor's update.
+static int64_t adam_groups(const GsoAdamTensor& a, bool sparse) {
+    const int64_t R = a.width < SPARSE_CHUNK ? SPARSE_CHUNK / a.width : 1;
+    return sparse ? (a.rows + R - 1) / R : (a.rows * a.width + ADAM_CHUNK - 1) / ADAM_CHUNK;
 }
 
 hipError_t launch_adam_clipped(int ngrads, const void* const* grads, const int64_t* numels, const int* types, int n,
@@ -620,17 +661,20 @@ hipError_t launch_adam_clipped(int ngrads, const void* const* grads, const int64
                                bool norm_known, void* temp, float* norm, hipStream_t st) {
     Coefficient c;
     bool scaled;
+    int64_t all = 0;
+    for (int i = 0; i < n; ++i) all += adam_groups(tensors[i], visible != nullptr);
     hipError_t e = norm_known ? launch_coefficient(kind, max_norm, temp, norm, st, &c)
-                              : launch_norm_for(NORM_STEP, ngrads, grads, numels, types, kind, max_norm, temp, norm, st, &c, &scaled);
+                              : launch_norm_for(NORM_STEP, ngrads, grads, numels, types, kind, max_norm, all, temp, norm, st, &c,
+                                                &scaled);
     for (int i = 0; i < n && e == hipSuccess;) {
         AdamTable t;
         t.n = 0;
         int64_t groups = 0;
         for (; i < n && t.n < ADAM_TABLE; ++i) {
             const GsoAdamTensor& a = tensors[i];
-            const int64_t numel = a.rows * a.width, R = a.width < SPARSE_CHUNK ? SPARSE_CHUNK / a.width : 1;
+            const int64_t numel = a.rows * a.width;
             if (numel <= 0) continue;
-            const int64_t more = visible ? (a.rows + R - 1) / R : (numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
+            const int64_t more = adam_groups(a, visible != nullptr);
             if (t.n > 0 && groups + more > 0x7fffffff) break;
             t.e[t.n] = {a.param, a.exp_avg, a.exp_avg_sq, a.grad, visible ? a.rows : numel, (uint32_t)a.width,
                         adam_const(a.lr, a.beta1, a.beta2, a.eps, a.bias_correction1, a.bias_correction2_sqrt)};
