@@ -31,8 +31,9 @@ struct WeightArgs {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// Four Gaussians a thread where every pointer allows 16-byte accesses.  Eight views' loads are issued before the first
-// of them is added.
+// Bound by its reads, 4 bytes a view and Gaussian.  Four Gaussians a thread where every pointer allows 16-byte accesses;
+// the loads of eight views are issued before the first is added, non-temporal because a view's weights are read once
+// (8 views of 6 M Gaussians: 43 us, 6.1 TB/s; 50 us with ordinary loads, 75 with one Gaussian a thread).
 template <int VEC>
 __global__ void __launch_bounds__(256) accumulate_weights_kernel(const WeightArgs a) {
     typedef float vec __attribute__((ext_vector_type(VEC)));
@@ -49,15 +50,14 @@ __global__ void __launch_bounds__(256) accumulate_weights_kernel(const WeightArg
     }
     vec w = *reinterpret_cast<const vec*>(a.weights + i), o = 0.0f, s = 0.0f;
     if (a.opacity) o = *reinterpret_cast<const vec*>(a.opacity + i);
-    int v = 0;
-    for (; v + 8 <= a.views; v += 8) {
+    for (int v = 0; v < a.views; v += 8) {
         vec c[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) c[u] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(a.contribution[v + u] + i));
+        for (int u = 0; u < 8; ++u)
+            c[u] = v + u < a.views ? __builtin_nontemporal_load(reinterpret_cast<const vec*>(a.contribution[v + u] + i)) : vec(0.0f);
 #pragma unroll
         for (int u = 0; u < 8; ++u) s += c[u];
     }
-    for (; v < a.views; ++v) s += *reinterpret_cast<const vec*>(a.contribution[v] + i);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         if (a.opacity) s[j] /= 1.0f + expf(-o[j]);
@@ -131,10 +131,13 @@ __device__ __forceinline__ uint2 find_bin(const uint32_t* hist, uint2 at) {
     return s_found;
 }
 
-constexpr int HIST_COPIES = 4;   // of the workgroup's histogram, side by side: few bins hold most weights
+// Copies of the workgroup's histogram, side by side, a quarter of the lanes each: few bins hold most weights (20 M rows of
+// one weight: 117 us for the selection, 267 with a single copy; of random weights 100 us either way).
+constexpr int HIST_COPIES = 4;
 
-// VECS: 16-byte loads a thread has in flight.  The rows that no view has seen all weigh zero; they are counted per wave
-// with a ballot, and only the others go to LDS.
+// One pass of the radix select, bound by reading the weights: 17.8 us for 20 M (4.5 TB/s, 3 us of it the launch, the bin
+// search and the merge).  VECS: 16-byte loads a thread has in flight.  The rows that no view has seen all weigh zero;
+// they are counted per wave with a ballot, and only the others go to LDS.
 template <int PASS, int VECS>
 __global__ void __launch_bounds__(HIST_THREADS) select_hist_kernel(int64_t old, const float* __restrict__ weights,
                                                                    SelectState* __restrict__ s) {
@@ -235,7 +238,8 @@ __device__ __forceinline__ RowBits row_bits(int64_t i, int64_t N, int64_t old, c
     return r;
 }
 
-// Per workgroup, a run of `tiles` tiles: rows above the threshold and rows that equal it, counted per wave with ballots.
+// Per workgroup, a run of `tiles` tiles: rows above the threshold and rows that equal it, counted per wave with ballots
+// (20 M rows: 16.8 us, 4.8 TB/s).
 __global__ void __launch_bounds__(SELECT_THREADS) select_count_kernel(int64_t N, int64_t old, int tiles,
                                                                       const float* __restrict__ weights,
                                                                       SelectState* __restrict__ s, uint2* __restrict__ counts) {
@@ -282,7 +286,8 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_count_kernel(int64_t N,
     }
 }
 
-// The kept rows of a tile are gathered in LDS and leave in one run: a thread's own sixteen would be stored 64 bytes apart.
+// The kept rows of a tile are gathered in LDS and leave in one run: a thread's own sixteen would be stored 64 bytes apart
+// (16 M of 20 M rows: 27 us, 5.3 TB/s of reads and writes; 49 us without).
 __global__ void __launch_bounds__(SELECT_THREADS) select_write_kernel(int64_t N, int64_t old, int tiles,
                                                                       const float* __restrict__ weights,
                                                                       const SelectState* __restrict__ s,
@@ -338,7 +343,8 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_write_kernel(int64_t N,
     }
 }
 
-// The whole selection in one workgroup, the keys in registers: one launch, which is what a small model's costs.
+// The whole selection in one workgroup, the keys in registers: one launch, which is what a small model's costs (5000 rows:
+// 10.7 us a call, six launches 19; with sixteen keys a thread 16384 rows take 22 us, more than the six launches).
 constexpr int SMALL_THREADS = 1024;
 constexpr int SMALL_PER = 8;
 constexpr int SMALL_ROWS = SMALL_PER * SMALL_THREADS;
@@ -456,7 +462,9 @@ template <typename T>
 using vector_of = f32x4 __attribute__((aligned(sizeof(T))));
 
 // At most two rows in a vector.  Four vectors are in flight per thread, and all row numbers are read before the first of
-// them: loads return in order, and a row number behind a vector would wait for it.
+// them: loads return in order, and a row number behind a vector would wait for it.  Four of five of 2.5 M rows: 45 floats
+// 5.5 TB/s of reads and writes, 3 floats 4.8 (3.5 with row numbers between the vectors, 3.5 with four 4-byte loads for
+// a vector, 2.6 with a float a thread).
 template <typename T>
 __device__ __forceinline__ void copy_wide(const RowRun& s, T* __restrict__ dst, uint32_t vectors) {
     constexpr uint32_t N = 16 / sizeof(T);
