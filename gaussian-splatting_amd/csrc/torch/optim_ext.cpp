@@ -42,6 +42,31 @@ int type_of(const Tensor& t, const char* what) {
     return 0;
 }
 
+// The values that a tensor stands for in its memory (a lazy conjugate or negative has others there).
+Tensor plain(const Tensor& t) { return t.is_conj() || t.is_neg() ? t.resolve_conj().resolve_neg() : t; }
+
+// Memory that a call writes must not overlap any other that it uses: the kernels work on all tensors at once.
+struct Spans {
+    struct Span {
+        uintptr_t begin, end;
+        bool written;
+    };
+    std::vector<Span> all;
+    void add(const void* p, int64_t bytes, bool written) {
+        if (bytes > 0) all.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written});
+    }
+    bool disjoint() {
+        std::sort(all.begin(), all.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+        uintptr_t end = 0, written_end = 0;
+        for (const Span& s : all) {
+            if (s.begin < (s.written ? end : written_end)) return false;
+            end = std::max(end, s.end);
+            if (s.written) written_end = std::max(written_end, s.end);
+        }
+        return true;
+    }
+};
+
 // The gradients of a list of parameters as the C ABI takes them.  A gradient whose elements do not fill a block of
 // memory of their own (a slice of something wider) is worked on in a packed copy.
 struct Grads {
@@ -72,7 +97,7 @@ Grads collect(const std::vector<Tensor>& params, const char* what) {
                     g.own.empty() ? t.device() : g.own[0].device(), " and ", t.device());
         g.type.push_back(type_of(t, what));
         g.own.push_back(t);
-        g.packed.push_back(t.is_non_overlapping_and_dense() ? t : t.contiguous());
+        g.packed.push_back(t.is_non_overlapping_and_dense() && !t.is_neg() ? t : plain(t).contiguous());
         g.ptr.push_back(g.packed.back().data_ptr());
         g.numel.push_back(g.packed.back().numel());
     }
@@ -81,22 +106,18 @@ Grads collect(const std::vector<Tensor>& params, const char* what) {
 
 // Scaling in place needs every element once: two gradients in the same memory would race.
 void check_disjoint(const Grads& g, const char* what) {
-    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-    spans.reserve(g.own.size());
+    Spans spans;
+    spans.all.reserve(g.own.size());
     for (size_t i = 0; i < g.own.size(); ++i) {
-        if (!g.packed[i].is_same(g.own[i])) {
-            for (int64_t d = 0; d < g.own[i].dim(); ++d)
-                TORCH_CHECK(g.own[i].stride(d) != 0 || g.own[i].size(d) <= 1, what,
-                            ": a gradient has several elements in one place (an expanded tensor)");
-        } else if (g.numel[i] > 0) {
-            const uintptr_t at = (uintptr_t)g.ptr[i];
-            spans.emplace_back(at, at + (uintptr_t)g.numel[i] * g.own[i].element_size());
+        if (g.packed[i].is_same(g.own[i])) {
+            spans.add(g.ptr[i], g.numel[i] * g.own[i].element_size(), true);
+            continue;
         }
+        for (int64_t d = 0; d < g.own[i].dim(); ++d)
+            TORCH_CHECK(g.own[i].stride(d) != 0 || g.own[i].size(d) <= 1, what,
+                        ": a gradient has several elements in one place (an expanded tensor)");
     }
-    std::sort(spans.begin(), spans.end());
-    for (size_t i = 1; i < spans.size(); ++i)
-        TORCH_CHECK(spans[i].first >= spans[i - 1].second, what,
-                    ": two gradients share memory (is a parameter listed twice?)");
+    TORCH_CHECK(spans.disjoint(), what, ": two gradients share memory (is a parameter listed twice?)");
 }
 
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
@@ -190,6 +211,7 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
     std::vector<GsoAdamTensor> table;
     std::vector<Tensor> keep;
     std::vector<size_t> counted;
+    Spans spans;
     table.reserve(n);
     for (size_t i = 0; i < n; ++i) {
         const Tensor& p = params[i];
@@ -214,7 +236,9 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
             counted.push_back(i);
         }
         if (p.numel() == 0) continue;
-        keep.push_back(g.own[i].contiguous());
+        TORCH_CHECK(!p.is_neg() && !exp_avg[i].is_neg() && !exp_avg_sq[i].is_neg(), what, ": parameters and moments must hold "
+                    "their own values");
+        keep.push_back(plain(g.own[i]).contiguous());
         a.param = p.data_ptr<float>();
         a.grad = keep.back().data_ptr<float>();
         a.exp_avg = exp_avg[i].data_ptr<float>();
@@ -222,7 +246,13 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
         a.rows = rows;
         a.width = p.numel() / rows;
         table.push_back(a);
+        const int64_t bytes = p.numel() * (int64_t)sizeof(float);
+        spans.add(a.param, bytes, true);
+        spans.add(a.exp_avg, bytes, true);
+        spans.add(a.exp_avg_sq, bytes, true);
+        spans.add(a.grad, bytes, false);
     }
+    TORCH_CHECK(spans.disjoint(), what, ": a parameter or moment shares memory with another tensor of the step");
     void* st = stream_on(dev);
     Norm r(g);
     if (error_if_nonfinite) r.look(g, kind, st, what);
@@ -254,19 +284,18 @@ void accumulate_weights(const Tensor& weights, const std::vector<Tensor>& contri
         TORCH_CHECK(t.is_cuda() && t.device() == weights.device() && t.scalar_type() == torch::kFloat32 && t.numel() == N &&
                         t.dim() >= 1 && t.size(0) == N, what, ": ", name, " must be a float32 GPU tensor with one entry per "
                     "Gaussian (", N, ") on the weights' device, got ", t.sizes(), " ", t.scalar_type(), " on ", t.device());
-        keep.push_back(t.contiguous());
+        keep.push_back(plain(t).contiguous());
         return keep.back().data_ptr<float>();
     };
     take(weights, "weights");
-    TORCH_CHECK(weights.is_contiguous(), what, ": weights are updated in place and must be contiguous");
+    TORCH_CHECK(weights.is_contiguous() && !weights.is_neg(), what, ": weights are updated in place and must be contiguous");
     TORCH_CHECK(std::isfinite(decay), what, ": decay must be finite, got ", decay);
     for (const Tensor& c : contributions) ptr.push_back(take(c, "a contribution"));
     const float* o = opacity ? take(*opacity, "opacity") : nullptr;
     if (N == 0) return;
-    const uintptr_t w0 = (uintptr_t)weights.data_ptr(), w1 = w0 + (uintptr_t)N * 4;
-    for (size_t i = 1; i < keep.size(); ++i)
-        TORCH_CHECK((uintptr_t)keep[i].data_ptr() >= w1 || (uintptr_t)keep[i].data_ptr() + (uintptr_t)N * 4 <= w0, what,
-                    ": weights must not share memory with what is added to them");
+    Spans spans;
+    for (size_t i = 0; i < keep.size(); ++i) spans.add(keep[i].data_ptr(), N * (int64_t)sizeof(float), i == 0);
+    TORCH_CHECK(spans.disjoint(), what, ": weights must not share memory with what is added to them");
     c10::DeviceGuard guard(weights.device());
     check_rc(gso_accumulate_weights(N, weights.data_ptr<float>(), (int)ptr.size(), ptr.data(), o, decay,
                                     stream_on(weights.device())), what);
@@ -284,7 +313,7 @@ Tensor evict_select(const Tensor& weights, int64_t budget, int64_t recent) {
     TORCH_CHECK(recent >= 0 && recent <= budget, what, ": recent must lie between 0 and the budget (", budget, "), got ",
                 recent);
     c10::DeviceGuard guard(weights.device());
-    const Tensor w = weights.contiguous();
+    const Tensor w = plain(weights).contiguous();
     Tensor rows = torch::empty({std::min(N, budget)}, w.options().dtype(torch::kInt32));
     if (rows.numel() == 0) return rows;
     const size_t bytes = gso_evict_temp_bytes(N);
@@ -301,9 +330,11 @@ std::vector<Tensor> take_rows(const std::vector<Tensor>& tensors, const Tensor& 
     std::vector<Tensor> out, keep;
     std::vector<GsoRowCopy> copies;
     out.reserve(tensors.size());
-    for (const Tensor& t : tensors) {
-        TORCH_CHECK(t.layout() == c10::kStrided && t.device() == rows.device() && t.dim() >= 1 && t.size(0) == N, what,
-                    ": every tensor needs one row per weight (", N, ") on ", rows.device(), ", got ", t.sizes(), " on ", t.device());
+    for (const Tensor& own : tensors) {
+        TORCH_CHECK(own.layout() == c10::kStrided && own.device() == rows.device() && own.dim() >= 1 && own.size(0) == N, what,
+                    ": every tensor needs one row per weight (", N, ") on ", rows.device(), ", got ", own.sizes(), " on ",
+                    own.device());
+        const Tensor t = plain(own);
         // rows that are packed in themselves may lie any distance apart; others are packed first
         const Tensor s = t.is_contiguous() || (N > 0 && t.numel() > 0 && t.select(0, 0).is_contiguous()) ? t : t.contiguous();
         std::vector<int64_t> shape = s.sizes().vec();

@@ -442,7 +442,7 @@ def evict_rows(weights, budget, recent=0, tensors=()):
     beforehand, so unlike `RowCompactor` the host never waits.  `weights`: [N] or [N, 1], float32, on the GPU."""
     host = _host()
     rows = host.evict_select(weights, int(budget), int(recent))
-    return rows, host.take_rows(list(tensors), rows, weights.numel())
+    return rows, host.take_rows(_tensors(tensors), rows, weights.numel())
 
 
 @torch.no_grad()

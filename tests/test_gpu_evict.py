@@ -388,3 +388,20 @@ def test_two_evictions_at_once_on_two_streams():
     torch.cuda.synchronize()
     for w, t, (rows, kept) in zip(ws, ts, out):
         assert np.array_equal(rows.cpu().numpy(), _reference(w, 150_000, 1000)) and torch.equal(kept[0], t[rows.long()])
+
+
+def test_lazy_conjugates_and_a_single_tensor():
+    import gsplat_optim as G
+    z = torch.randn(100, 3, device="cuda", dtype=torch.complex64)
+    w = torch.rand(100, device="cuda")
+    rows, kept = G.evict_rows(w, 60, 0, [z.conj(), z.conj().imag, z.conj().real])
+    at = rows.long()
+    assert torch.equal(kept[0], z[at].conj()) and torch.equal(kept[1], -z.imag[at]) and torch.equal(kept[2], z.real[at])
+    rows, kept = G.evict_rows(w, 60, 0, z)
+    assert len(kept) == 1 and torch.equal(kept[0], z[rows.long()])
+    lazy = torch.complex(w, -w).conj().imag
+    assert lazy.is_neg() is True
+    assert np.array_equal(G.evict_rows(lazy, 60)[0].cpu().numpy(), _reference(w, 60, 0))
+    acc = torch.zeros(100, device="cuda")
+    G.accumulate_weights(acc, [lazy])
+    assert torch.equal(acc, w)

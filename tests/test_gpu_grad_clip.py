@@ -479,3 +479,38 @@ def test_two_calls_at_once_on_two_streams():
     torch.cuda.synchronize()
     for k in range(2):
         assert torch.equal(got[k], norms[k]) and all(torch.equal(a, b) for a, b in zip(sets[k], want[k]))
+
+
+def test_tensors_of_a_step_must_not_share_memory():
+    import gsplat_optim as G
+    flat = torch.ones(300, device="cuda")
+    p, q = torch.nn.Parameter(flat[:200].view(100, 2)), torch.nn.Parameter(flat[150:250].view(50, 2))
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    opt = G.FusedGaussianAdam([p, q], lr=0.1)
+    with pytest.raises(RuntimeError, match="shares memory"):
+        opt.clipped_step(1.0)
+    assert len(opt.state) == 0 and bool((flat == 1).all())
+    a, b = torch.nn.Parameter(torch.ones(10, device="cuda")), torch.nn.Parameter(torch.ones(10, device="cuda"))
+    a.grad = b.grad = torch.ones(10, device="cuda")          # read by both: allowed
+    G.FusedGaussianAdam([a, b], lr=0.1).clipped_step(1e9)
+    assert torch.equal(a, b) and float(a[0]) < 1
+    with pytest.raises(RuntimeError, match="shares memory"):
+        a.grad = b.data
+        G.FusedGaussianAdam([a, b], lr=0.1).clipped_step(1e9)
+
+
+def test_lazy_negatives_count_as_what_they_stand_for():
+    import gsplat_optim as G
+    z = torch.complex(torch.randn(50, device="cuda"), torch.rand(50, device="cuda") + 1)
+    g = z.conj().imag
+    assert g.is_neg()
+    p = torch.nn.Parameter(torch.ones(50, device="cuda"))
+    p.grad = g.clone()
+    want = torch.nn.Parameter(torch.ones(50, device="cuda"))
+    want.grad = p.grad
+    lazy = torch.nn.Parameter(torch.ones(50, device="cuda"))
+    lazy.grad = g
+    a, b = G.FusedGaussianAdam([want], lr=0.1), G.FusedGaussianAdam([lazy], lr=0.1)
+    assert torch.equal(a.clipped_step(1.0), b.clipped_step(1.0)) and torch.equal(want, lazy)
+    n = float(G.clip_grad_norm_(lazy, 0.5))
+    assert torch.allclose(g, want.grad * (0.5 / (n + 1e-6)), rtol=1e-6)
