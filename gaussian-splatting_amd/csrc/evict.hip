@@ -11,9 +11,11 @@
 //
 // The number of kept rows is known before any row is looked at, so nothing here
 // makes the host wait.  The k-th largest weight is found by a radix select on
-// the weights' bits (three histograms of 11, 11 and 10 bits), then one pass
-// counts and one writes the kept rows in ascending order.  All counts are
-// integers: the result is the same in every run.
+// the weights' bits (three histograms of 11, 11 and 10 bits).  The third pass
+// knows 22 of them and leaves two bits per row: above all weights with these 22
+// bits, or one of them.  Counting and writing the kept rows reads those bits, and
+// the weights of the rows among the second only.  All counts are integers: the
+// result is the same in every run.
 #include "kernels.h"
 
 namespace gs {
@@ -80,6 +82,13 @@ struct SelectState {
                       // that equal them are still to be kept
 };
 
+// Two bits of every row, a segment of 256 rows in eight words: bit l of word j is row 4 l + j of the segment, as a ballot
+// over lanes with four rows each gives it.
+constexpr int SEGMENT = 256;
+struct SegmentBits {
+    uint64_t above[4], level[4];
+};
+
 // Unsigned integers that order as the weights do: NaN lowest, then -inf .. +inf, and -0 equal to +0.
 __device__ __forceinline__ uint32_t weight_key(float w) {
     if (w != w) return 0u;
@@ -136,11 +145,12 @@ __device__ __forceinline__ uint2 find_bin(const uint32_t* hist, uint2 at) {
 constexpr int HIST_COPIES = 4;
 
 // One pass of the radix select, bound by reading the weights: 17.8 us for 20 M (4.5 TB/s, 3 us of it the launch, the bin
-// search and the merge).  VECS: 16-byte loads a thread has in flight.  The rows that no view has seen all weigh zero;
+// search and the merge; the third, which leaves the rows' bits, 20.5).  VECS: 16-byte loads a thread has in flight.  The rows that no view has seen all weigh zero;
 // they are counted per wave with a ballot, and only the others go to LDS.
 template <int PASS, int VECS>
 __global__ void __launch_bounds__(HIST_THREADS) select_hist_kernel(int64_t old, const float* __restrict__ weights,
-                                                                   SelectState* __restrict__ s) {
+                                                                   SelectState* __restrict__ s,
+                                                                   SegmentBits* __restrict__ segments) {
     __shared__ uint32_t h[HIST_BINS * HIST_COPIES];
     constexpr int shift = pass_shift(PASS), bits = pass_bits(PASS), step = 4 * VECS * HIST_THREADS;
     constexpr uint32_t ZERO = 0x80000000u;   // weight_key(0)
@@ -158,36 +168,55 @@ __global__ void __launch_bounds__(HIST_THREADS) select_hist_kernel(int64_t old, 
     uint32_t* own = h + (threadIdx.x & (HIST_COPIES - 1));
     const bool count_zeros = PASS == 0 || (uint32_t)((uint64_t)ZERO >> (shift + bits)) == prefix;
     uint32_t zeros = 0;
-    auto add = [&](float w, bool valid) {
-        const uint32_t k = weight_key(w);
-        bool in = valid && (PASS == 0 || (uint32_t)((uint64_t)k >> (shift + bits)) == prefix);
-        if (count_zeros) {
-            zeros += (uint32_t)__popcll(__ballot(valid && k == ZERO));
-            in = in && k != ZERO;
+    const int lane = threadIdx.x & (WAVE - 1);
+    // four rows of a lane, `valid` of them
+    auto add = [&](const f32x4& w, int64_t i, int valid) {
+        uint64_t word[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t k = weight_key(w[j]), top = (uint32_t)((uint64_t)k >> (shift + bits));
+            bool in = j < valid && (PASS == 0 || top == prefix);
+            if (PASS == 2) {
+                word[j] = __ballot(j < valid && top > prefix);
+                word[4 + j] = __ballot(in);
+            }
+            if (count_zeros) {
+                zeros += (uint32_t)__popcll(__ballot(j < valid && k == ZERO));
+                in = in && k != ZERO;
+            }
+            if (in) atomicAdd(own + ((k >> shift) & ((1u << bits) - 1)) * HIST_COPIES, 1u);
         }
-        if (in) atomicAdd(own + ((k >> shift) & ((1u << bits) - 1)) * HIST_COPIES, 1u);
+        if (PASS == 2) {
+            uint64_t mine = word[0];   // lane x stores word x
+#pragma unroll
+            for (int x = 1; x < 8; ++x) mine = lane == x ? word[x] : mine;
+            const int64_t first = i - 4 * lane;   // of the wave's segment
+            if (lane < 8 && first < old)
+                reinterpret_cast<uint64_t*>(segments + first / SEGMENT)[lane] = mine;
+        }
     };
     const bool aligned = ((uintptr_t)weights & 15) == 0;
     for (int64_t base = (int64_t)blockIdx.x * step; base < old; base += (int64_t)gridDim.x * step) {
+        const int64_t i0 = base + 4 * (int)threadIdx.x;
         if (aligned && base + step <= old) {
-            const f32x4* p = reinterpret_cast<const f32x4*>(weights + base) + threadIdx.x;
             f32x4 w[VECS];
 #pragma unroll
-            for (int q = 0; q < VECS; ++q) w[q] = p[q * HIST_THREADS];
+            for (int q = 0; q < VECS; ++q) w[q] = *reinterpret_cast<const f32x4*>(weights + i0 + 4 * q * HIST_THREADS);
 #pragma unroll
-            for (int q = 0; q < VECS; ++q)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) add(w[q][j], true);
+            for (int q = 0; q < VECS; ++q) add(w[q], i0 + 4 * q * HIST_THREADS, 4);
         } else {
-            const int count = old - base < step ? (int)(old - base) : step;
-            for (int i0 = 0; i0 < count; i0 += HIST_THREADS) {
-                const int i = i0 + (int)threadIdx.x;
-                add(i < count ? weights[base + i] : 0.0f, i < count);
+            for (int q = 0; q < VECS; ++q) {
+                const int64_t i = i0 + 4 * q * HIST_THREADS;
+                const int valid = old - i >= 4 ? 4 : old > i ? (int)(old - i) : 0;
+                f32x4 w = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < valid) w[j] = weights[i + j];
+                add(w, i, valid);
             }
         }
     }
-    if (zeros && (threadIdx.x & 63) == 0)
-        atomicAdd(own + ((ZERO >> shift) & ((1u << bits) - 1)) * HIST_COPIES, zeros);
+    if (zeros && lane == 0) atomicAdd(own + ((ZERO >> shift) & ((1u << bits) - 1)) * HIST_COPIES, zeros);
     __syncthreads();
     for (int b = threadIdx.x; b < HIST_BINS; b += HIST_THREADS) {
         uint32_t n = 0;
@@ -206,79 +235,83 @@ __device__ __forceinline__ uint32_t block_sum_u32(uint32_t v, uint32_t* s_w) {
     return s_w[0] + s_w[1] + s_w[2] + s_w[3];
 }
 
-// Sixteen rows of a thread, one bit each: above the threshold (the recent rows among them), and equal to it.
-struct RowBits {
-    uint32_t above, level;
+// The threshold of a finished select, and whether all rows that share its upper 22 bits equal it (ties at zero, or one row):
+// then the bits alone tell what is kept.
+struct Threshold {
+    uint32_t key, need;
+    bool one;
 };
-__device__ __forceinline__ RowBits row_bits(int64_t i, int64_t N, int64_t old, const float* __restrict__ weights, uint32_t key,
-                                            bool aligned) {
-    RowBits r = {0, 0};
-    if (aligned && i + 16 <= old) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(weights + i + 4 * q);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t k = weight_key(x[j]);
-                r.above |= (k > key ? 1u : 0u) << (4 * q + j);
-                r.level |= (k == key ? 1u : 0u) << (4 * q + j);
-            }
-        }
-    } else {
-        for (int j = 0; j < 16 && i + j < N; ++j) {
-            if (i + j >= old) {
-                r.above |= 1u << j;
-            } else {
-                const uint32_t k = weight_key(weights[i + j]);
-                r.above |= (k > key ? 1u : 0u) << j;
-                r.level |= (k == key ? 1u : 0u) << j;
-            }
-        }
-    }
-    return r;
+__device__ __forceinline__ Threshold threshold_of(const SelectState* __restrict__ s, uint2 at) {
+    return {at.x, at.y, s->hist[2][at.x & 1023u] == s->hist[1][s->at[2].x & 2047u]};
 }
 
-// Per workgroup, a run of `tiles` tiles: rows above the threshold and rows that equal it, counted per wave with ballots
-// (20 M rows: 16.8 us, 4.8 TB/s).
-__global__ void __launch_bounds__(SELECT_THREADS) select_count_kernel(int64_t N, int64_t old, int tiles,
-                                                                      const float* __restrict__ weights,
-                                                                      SelectState* __restrict__ s, uint2* __restrict__ counts) {
-    __shared__ uint2 s_w[SELECT_THREADS / WAVE];
-    const uint2 at = find_bin<2, SELECT_THREADS>(s->hist[2], s->at[2]);
-    if (blockIdx.x == 0 && threadIdx.x == 0) s->at[3] = at;
-    const bool aligned = ((uintptr_t)weights & 15) == 0;
-    uint32_t above = 0, level = 0;
-    auto add = [&](float w, bool valid) {
-        const uint32_t k = weight_key(w);
-        above += (uint32_t)__popcll(__ballot(valid && k > at.x));
-        level += (uint32_t)__popcll(__ballot(valid && k == at.x));
-    };
-    const int64_t begin = (int64_t)blockIdx.x * tiles * SELECT_ROWS;
-    int64_t end = begin + (int64_t)tiles * SELECT_ROWS;
-    if (end > N) end = N;
-    const int64_t stop = end < old ? end : old;   // the recent rows behind are kept unseen
-    int64_t base = begin;
-    if (aligned) {
-        for (; base + SELECT_ROWS <= stop; base += SELECT_ROWS) {
-            const f32x4* p = reinterpret_cast<const f32x4*>(weights + base) + threadIdx.x;
-            f32x4 w[4];
+// A lane's bit of a word that is the same in all lanes.
+__device__ __forceinline__ bool lane_bit(uint64_t word) { return __builtin_amdgcn_inverse_ballot_w64(word); }
+
+// A segment's rows above the threshold (the recent ones among them) and at it, for a wave.
+__device__ __forceinline__ SegmentBits load_segment(int64_t segment, int64_t old, const SegmentBits* __restrict__ segments) {
+    SegmentBits b = {};
+    if (segment * SEGMENT < old) b = segments[segment];
+    return b;
+}
+__device__ __forceinline__ void resolve_segment(SegmentBits& b, int64_t segment, int64_t N, int64_t old,
+                                                const float* __restrict__ weights, const Threshold& t) {
+    const int64_t first = segment * SEGMENT, i = first + 4 * (int)(threadIdx.x & (WAVE - 1));
+    if (!t.one && (b.level[0] | b.level[1] | b.level[2] | b.level[3]) != 0) {
+        float w[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) w[q] = p[q * SELECT_THREADS];
+        for (int j = 0; j < 4; ++j) w[j] = lane_bit(b.level[j]) ? weights[i + j] : 0.0f;
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) add(w[q][j], true);
+        for (int j = 0; j < 4; ++j) {
+            const bool in = lane_bit(b.level[j]);
+            const uint32_t k = weight_key(w[j]);
+            b.above[j] |= __ballot(in && k > t.key);
+            b.level[j] = __ballot(in && k == t.key);
         }
     }
-    for (; base < stop; base += SELECT_THREADS) {
-        const int64_t i = base + (int)threadIdx.x;
-        add(i < stop ? weights[i] : 0.0f, i < stop);
+    if (first + SEGMENT > old) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b.above[j] |= __ballot(i + j >= old && i + j < N);
     }
-    if ((threadIdx.x & 63) == 0) s_w[threadIdx.x >> 6] = make_uint2(above, level);
+}
+__device__ __forceinline__ uint32_t count_rows(const uint64_t (&word)[4]) {
+    return (uint32_t)(__popcll(word[0]) + __popcll(word[1]) + __popcll(word[2]) + __popcll(word[3]));
+}
+
+constexpr int SELECT_WAVES = SELECT_THREADS / WAVE;
+constexpr int WAVE_SEGMENTS = SELECT_ROWS / SEGMENT / SELECT_WAVES;   // of a tile
+
+// Per workgroup, a run of `tiles` tiles: rows above the threshold and rows that equal it (20 M rows: 9.6 us, 16.8 when it
+// read the weights).
+__global__ void __launch_bounds__(SELECT_THREADS) select_count_kernel(int64_t N, int64_t old, int tiles,
+                                                                      const float* __restrict__ weights,
+                                                                      SelectState* __restrict__ s,
+                                                                      const SegmentBits* __restrict__ segments,
+                                                                      uint2* __restrict__ counts) {
+    __shared__ uint2 s_w[SELECT_WAVES];
+    const uint2 at = find_bin<2, SELECT_THREADS>(s->hist[2], s->at[2]);
+    if (blockIdx.x == 0 && threadIdx.x == 0) s->at[3] = at;
+    const Threshold t = threshold_of(s, at);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
+    uint32_t above = 0, level = 0;
+    const int64_t first = (int64_t)blockIdx.x * tiles * (SELECT_ROWS / SEGMENT), all = (N + SEGMENT - 1) / SEGMENT;
+    const int64_t end = first + tiles * (SELECT_ROWS / SEGMENT) < all ? first + tiles * (SELECT_ROWS / SEGMENT) : all;
+    for (int64_t x = first + wave * WAVE_SEGMENTS; x < end; x += SELECT_WAVES * WAVE_SEGMENTS) {
+        SegmentBits b[WAVE_SEGMENTS];   // the loads of all of them first
+#pragma unroll
+        for (int y = 0; y < WAVE_SEGMENTS; ++y) b[y] = load_segment(x + y, old, segments);
+#pragma unroll
+        for (int y = 0; y < WAVE_SEGMENTS; ++y) {
+            resolve_segment(b[y], x + y, N, old, weights, t);
+            above += count_rows(b[y].above);
+            level += count_rows(b[y].level);
+        }
+    }
+    if ((threadIdx.x & 63) == 0) s_w[wave] = make_uint2(above, level);
     __syncthreads();
     if (threadIdx.x == 0) {
-        uint2 c = make_uint2(end > old ? (uint32_t)(end - (begin > old ? begin : old)) : 0u, 0u);
-        for (int w = 0; w < SELECT_THREADS / WAVE; ++w) {
+        uint2 c = make_uint2(0u, 0u);
+        for (int w = 0; w < SELECT_WAVES; ++w) {
             c.x += s_w[w].x;
             c.y += s_w[w].y;
         }
@@ -286,58 +319,115 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_count_kernel(int64_t N,
     }
 }
 
-// The kept rows of a tile are gathered in LDS and leave in one run: a thread's own sixteen would be stored 64 bytes apart
-// (16 M of 20 M rows: 27 us, 5.3 TB/s of reads and writes; 49 us without).
+// The bits of the words below a lane.
+__device__ __forceinline__ uint32_t count_below(const uint64_t (&word)[4]) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        n = __builtin_amdgcn_mbcnt_hi((uint32_t)(word[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)word[j], n));
+    return n;
+}
+
+// The kept rows of a tile are gathered in LDS and leave in one run (16 M of 20 M rows: 23 us, 34 with each lane storing its
+// own, 27 when it read the weights); bound by its stores, 64 MB, and the chain of loads in front of them.
 __global__ void __launch_bounds__(SELECT_THREADS) select_write_kernel(int64_t N, int64_t old, int tiles,
                                                                       const float* __restrict__ weights,
                                                                       const SelectState* __restrict__ s,
+                                                                      const SegmentBits* __restrict__ segments,
                                                                       const uint2* __restrict__ counts,
                                                                       int32_t* __restrict__ rows) {
     __shared__ uint32_t s_w[4];
-    __shared__ uint32_t s_scan[4];
-    __shared__ int32_t s_rows[SELECT_ROWS];
-    const uint32_t key = s->at[3].x, need = s->at[3].y;
+    __shared__ uint2 s_count[SELECT_WAVES];
+    __shared__ __attribute__((aligned(16))) int32_t s_rows[SELECT_ROWS + 4];
+    const Threshold t = threshold_of(s, s->at[3]);
+    const uint32_t need = t.need;
     uint32_t above = 0, level = 0;   // rows of the workgroups before this one
-    for (uint32_t b = threadIdx.x; b < blockIdx.x; b += SELECT_THREADS) {
-        above += counts[b].x;
-        level += counts[b].y;
+    {
+        constexpr int LOADS = SELECT_GROUPS / SELECT_THREADS;   // all at once
+        uint2 c[LOADS];
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const uint32_t b = u * SELECT_THREADS + threadIdx.x;
+            c[u] = b < blockIdx.x ? counts[b] : make_uint2(0u, 0u);
+        }
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            above += c[u].x;
+            level += c[u].y;
+        }
     }
     above = block_sum_u32(above, s_w);
     level = block_sum_u32(level, s_w);
-    const bool aligned = ((uintptr_t)weights & 15) == 0;
-    const int w = threadIdx.x >> 6;
-    for (int t = 0; t < tiles; ++t) {
-        const int64_t tile = ((int64_t)blockIdx.x * tiles + t) * SELECT_ROWS;
-        if (tile >= N) break;
-        const int64_t i = tile + 16 * (int)threadIdx.x;
-        RowBits r = {0, 0};
-        if (i < N) r = row_bits(i, N, old, weights, key, aligned);
-        // both counts of a tile fit 16 bits
-        const uint32_t own = (uint32_t)__popc(r.above) | (uint32_t)__popc(r.level) << 16;
-        const uint32_t incl = wave_scan_u32(own);
-        if ((threadIdx.x & 63) == 63) s_scan[w] = incl;
-        __syncthreads();
-        uint32_t before = incl - own;
-        for (int x = 0; x < w; ++x) before += s_scan[x];
-        const uint32_t tile_all = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
-        uint32_t pl = level + (before >> 16);                       // rows at the threshold before this thread's
-        const uint32_t level_at = level < need ? level : need;      // of them kept before the tile
-        uint32_t out = (before & 0xffffu) + (pl < need ? pl : need) - level_at;
-        const uint32_t any = r.above | r.level;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
+    for (int k = 0; k < tiles; ++k) {
+        const int64_t tile = (int64_t)blockIdx.x * tiles + k;
+        if (tile * SELECT_ROWS >= N) break;
+        const int64_t segment = tile * (SELECT_ROWS / SEGMENT) + wave * WAVE_SEGMENTS;
+        SegmentBits b[WAVE_SEGMENTS];
+        uint32_t na = 0, nl = 0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            if (any >> j & 1u) {
-                const bool l = r.level >> j & 1u;
-                if (!l || pl < need) s_rows[out++] = (int32_t)(i + j);
-                pl += l ? 1u : 0u;
+        for (int x = 0; x < WAVE_SEGMENTS; ++x) b[x] = load_segment(segment + x, old, segments);
+#pragma unroll
+        for (int x = 0; x < WAVE_SEGMENTS; ++x) {
+            resolve_segment(b[x], segment + x, N, old, weights, t);
+            na += count_rows(b[x].above);
+            nl += count_rows(b[x].level);
+        }
+        if ((threadIdx.x & 63) == 0) s_count[wave] = make_uint2(na, nl);
+        __syncthreads();
+        uint32_t pa = 0, pl = level, tile_above = 0, tile_level = 0;   // rows before the segment: above, in the tile; at the threshold
+        for (int w = 0; w < SELECT_WAVES; ++w) {
+            const uint2 c = s_count[w];
+            pa += w < wave ? c.x : 0u;
+            pl += w < wave ? c.y : 0u;
+            tile_above += c.x;
+            tile_level += c.y;
+        }
+        const uint32_t level_at = level < need ? level : need;   // rows at the threshold kept before the tile
+        const uint32_t level_end = level + tile_level;
+        const bool all_level = level_end <= need;
+        const uint32_t kept = tile_above + (all_level ? level_end : need) - level_at;
+        // the list starts where its first row falls in sixteen bytes of the output, so that it leaves in whole vectors
+        int32_t* to = rows + (above + level_at);
+        const uint32_t skip = (uint32_t)((uintptr_t)to >> 2) & 3u;
+        if (all_level || level >= need) {   // every tile but one: the rows at the threshold stay all, or go all
+            uint32_t out = skip + pa + (all_level ? pl - level : 0u);
+#pragma unroll
+            for (int x = 0; x < WAVE_SEGMENTS; ++x) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) b[x].above[j] |= all_level ? b[x].level[j] : 0ull;
+                uint32_t at = out + count_below(b[x].above);
+                const int32_t i = (int32_t)((segment + x) * SEGMENT) + 4 * (int)(threadIdx.x & (WAVE - 1));
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (lane_bit(b[x].above[j])) s_rows[at++] = i + j;
+                out += count_rows(b[x].above);
+            }
+        } else {
+#pragma unroll
+            for (int x = 0; x < WAVE_SEGMENTS; ++x) {
+                uint32_t n = pa + count_below(b[x].above), l = pl + count_below(b[x].level);
+                const int32_t i = (int32_t)((segment + x) * SEGMENT) + 4 * (int)(threadIdx.x & (WAVE - 1));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool is_above = lane_bit(b[x].above[j]), is_level = lane_bit(b[x].level[j]);
+                    if (is_above || (is_level && l < need)) s_rows[skip + n + (l < need ? l : need) - level_at] = i + j;
+                    n += is_above ? 1u : 0u;
+                    l += is_level ? 1u : 0u;
+                }
+                pa += count_rows(b[x].above);
+                pl += count_rows(b[x].level);
             }
         }
         __syncthreads();
-        const uint32_t level_end = level + (tile_all >> 16);
-        const uint32_t kept = (tile_all & 0xffffu) + (level_end < need ? level_end : need) - level_at;
-        const uint32_t to = above + level_at;
-        for (uint32_t x = threadIdx.x; x < kept; x += SELECT_THREADS) rows[to + x] = s_rows[x];
-        above += tile_all & 0xffffu;
+        const uint32_t end = skip + kept, vectors = end >> 2;
+        int4* out4 = reinterpret_cast<int4*>(to - skip);
+        for (uint32_t v = threadIdx.x + (skip ? 1u : 0u); v < vectors; v += SELECT_THREADS) out4[v] = reinterpret_cast<int4*>(s_rows)[v];
+        if (threadIdx.x < 8) {   // what is left of the first vector and of the last
+            const uint32_t x = threadIdx.x < 4 ? threadIdx.x : (vectors << 2) + threadIdx.x - 4;
+            if (x >= skip && x < end && (threadIdx.x < 4 ? skip != 0 && vectors > 0 : true)) to[x - skip] = s_rows[x];
+        }
+        above += tile_above;
         level = level_end;
         __syncthreads();
     }
@@ -585,22 +675,23 @@ hipError_t launch_accumulate_weights(int64_t N, float* weights, int views, const
     return hipGetLastError();
 }
 
+static size_t select_fixed_bytes() { return align_up(sizeof(SelectState), 256) + align_up(SELECT_GROUPS * sizeof(uint2), 256); }
+
 size_t evict_temp_bytes(int64_t N) {
-    (void)N;
-    return align_up(sizeof(SelectState), 256) + SELECT_GROUPS * sizeof(uint2);
+    return select_fixed_bytes() + (N > SMALL_ROWS ? (size_t)((N + SEGMENT - 1) / SEGMENT) * sizeof(SegmentBits) : 0);
 }
 
 // One vector a thread while that gives every workgroup at most one step, four from there on.
 template <int PASS>
-static void launch_hist(int64_t old, const float* weights, SelectState* s, hipStream_t st) {
+static void launch_hist(int64_t old, const float* weights, SelectState* s, SegmentBits* segments, hipStream_t st) {
     const int64_t steps = (old + 4 * HIST_THREADS - 1) / (4 * HIST_THREADS);
     if (steps <= HIST_GROUPS) {
-        hipLaunchKernelGGL((select_hist_kernel<PASS, 1>), dim3((unsigned)steps), dim3(HIST_THREADS), 0, st, old, weights, s);
+        hipLaunchKernelGGL((select_hist_kernel<PASS, 1>), dim3((unsigned)steps), dim3(HIST_THREADS), 0, st, old, weights, s, segments);
     } else {
         constexpr int VECS = 4;
         const int64_t wide = (steps + VECS - 1) / VECS;
         hipLaunchKernelGGL((select_hist_kernel<PASS, VECS>), dim3((unsigned)(wide < HIST_GROUPS ? wide : HIST_GROUPS)),
-                           dim3(HIST_THREADS), 0, st, old, weights, s);
+                           dim3(HIST_THREADS), 0, st, old, weights, s, segments);
     }
 }
 
@@ -621,15 +712,16 @@ hipError_t launch_evict_select(int64_t N, const float* weights, int64_t budget, 
     }
     SelectState* s = (SelectState*)temp;
     uint2* counts = (uint2*)((char*)temp + align_up(sizeof(SelectState), 256));
+    SegmentBits* segments = (SegmentBits*)((char*)temp + select_fixed_bytes());
     const int64_t all = (N + SELECT_ROWS - 1) / SELECT_ROWS;
     const int tiles = (int)((all + SELECT_GROUPS - 1) / SELECT_GROUPS);
     const dim3 groups((unsigned)((all + tiles - 1) / tiles));
     hipLaunchKernelGGL(select_clear_kernel, dim3(24), dim3(256), 0, st, s, (uint32_t)(keep - recent));
-    launch_hist<0>(old, weights, s, st);
-    launch_hist<1>(old, weights, s, st);
-    launch_hist<2>(old, weights, s, st);
-    hipLaunchKernelGGL(select_count_kernel, groups, dim3(SELECT_THREADS), 0, st, N, old, tiles, weights, s, counts);
-    hipLaunchKernelGGL(select_write_kernel, groups, dim3(SELECT_THREADS), 0, st, N, old, tiles, weights, s, counts, rows);
+    launch_hist<0>(old, weights, s, segments, st);
+    launch_hist<1>(old, weights, s, segments, st);
+    launch_hist<2>(old, weights, s, segments, st);
+    hipLaunchKernelGGL(select_count_kernel, groups, dim3(SELECT_THREADS), 0, st, N, old, tiles, weights, s, segments, counts);
+    hipLaunchKernelGGL(select_write_kernel, groups, dim3(SELECT_THREADS), 0, st, N, old, tiles, weights, s, segments, counts, rows);
     return hipGetLastError();
 }
 
