@@ -56,7 +56,8 @@ struct Spans {
         if (bytes > 0) all.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written});
     }
     bool disjoint() {
-        std::sort(all.begin(), all.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+        const auto before = [](const Span& a, const Span& b) { return a.begin < b.begin; };
+        if (!std::is_sorted(all.begin(), all.end(), before)) std::sort(all.begin(), all.end(), before);
         uintptr_t end = 0, written_end = 0;
         for (const Span& s : all) {
             if (s.begin < (s.written ? end : written_end)) return false;
@@ -67,13 +68,15 @@ struct Spans {
     }
 };
 
-// The gradients of a list of parameters as the C ABI takes them.  A gradient whose elements do not fill a block of
-// memory of their own (a slice of something wider) is worked on in a packed copy.
+// The gradients of a list of parameters as the C ABI takes them (the list outlives it).  A gradient whose elements do not
+// fill a block of memory of their own (a slice of something wider) is worked on in a packed copy.
 struct Grads {
-    std::vector<Tensor> own, packed;   // packed[i] is own[i], or the copy
+    std::vector<const Tensor*> own;
+    std::vector<std::pair<size_t, Tensor>> packed;   // (index, copy)
     std::vector<void*> ptr;
     std::vector<int64_t> numel;
     std::vector<int> type;
+    c10::Device device = c10::Device(c10::kCPU);
     int n() const { return (int)ptr.size(); }
     const void* const* cptr() const { return (const void* const*)ptr.data(); }
 };
@@ -83,7 +86,6 @@ Grads collect(const std::vector<Tensor>& params, const char* what) {
     Grads g;
     const size_t n = params.size();
     g.own.reserve(n);
-    g.packed.reserve(n);
     g.ptr.reserve(n);
     g.numel.reserve(n);
     g.type.reserve(n);
@@ -93,30 +95,32 @@ Grads collect(const std::vector<Tensor>& params, const char* what) {
         if (!t.defined()) continue;
         TORCH_CHECK(t.layout() == c10::kStrided, what, ": gradients must be dense, got layout ", t.layout());
         TORCH_CHECK(t.is_cuda(), what, ": gradients must be GPU tensors (there is no CPU path), got one on ", t.device());
-        TORCH_CHECK(g.own.empty() || t.device() == g.own[0].device(), what, ": gradients must be on one device, got ",
-                    g.own.empty() ? t.device() : g.own[0].device(), " and ", t.device());
+        if (g.own.empty()) g.device = t.device();
+        TORCH_CHECK(t.device() == g.device, what, ": gradients must be on one device, got ", g.device, " and ", t.device());
         g.type.push_back(type_of(t, what));
-        g.own.push_back(t);
-        g.packed.push_back(t.is_non_overlapping_and_dense() && !t.is_neg() ? t : plain(t).contiguous());
-        g.ptr.push_back(g.packed.back().data_ptr());
-        g.numel.push_back(g.packed.back().numel());
+        if (!t.is_non_overlapping_and_dense() || t.is_neg()) {
+            g.packed.emplace_back(g.own.size(), plain(t).contiguous());
+            g.ptr.push_back(g.packed.back().second.data_ptr());
+        } else {
+            g.ptr.push_back(t.data_ptr());
+        }
+        g.own.push_back(&t);
+        g.numel.push_back(t.numel());
     }
     return g;
 }
 
 // Scaling in place needs every element once: two gradients in the same memory would race.
 void check_disjoint(const Grads& g, const char* what) {
-    Spans spans;
-    spans.all.reserve(g.own.size());
-    for (size_t i = 0; i < g.own.size(); ++i) {
-        if (g.packed[i].is_same(g.own[i])) {
-            spans.add(g.ptr[i], g.numel[i] * g.own[i].element_size(), true);
-            continue;
-        }
-        for (int64_t d = 0; d < g.own[i].dim(); ++d)
-            TORCH_CHECK(g.own[i].stride(d) != 0 || g.own[i].size(d) <= 1, what,
+    for (const auto& copy : g.packed) {
+        const Tensor& t = *g.own[copy.first];
+        for (int64_t d = 0; d < t.dim(); ++d)
+            TORCH_CHECK(t.stride(d) != 0 || t.size(d) <= 1, what,
                         ": a gradient has several elements in one place (an expanded tensor)");
     }
+    Spans spans;
+    spans.all.reserve(g.own.size());
+    for (size_t i = 0; i < g.own.size(); ++i) spans.add(g.ptr[i], g.numel[i] * (g.type[i] == GSO_F32 ? 4 : 2), true);
     TORCH_CHECK(spans.disjoint(), what, ": two gradients share memory (is a parameter listed twice?)");
 }
 
@@ -131,7 +135,7 @@ struct Norm {
     Tensor temp, value;
     size_t bytes;
     explicit Norm(const Grads& g) : bytes(gso_norm_temp_bytes(g.n())) {
-        const auto opt = torch::TensorOptions().device(g.own[0].device());
+        const auto opt = torch::TensorOptions().device(g.device);
         temp = torch::empty({(int64_t)bytes}, opt.dtype(torch::kUInt8));
         value = torch::empty({}, opt.dtype(torch::kFloat32));
     }
@@ -153,9 +157,9 @@ Tensor grad_norm(const std::vector<Tensor>& params, double norm_type) {
     const int kind = norm_kind(norm_type, what);
     const Grads g = collect(params, what);
     if (g.own.empty()) return torch::zeros({});
-    c10::DeviceGuard guard(g.own[0].device());
+    c10::DeviceGuard guard(g.device);
     Norm r(g);
-    r.form(g, kind, stream_on(g.own[0].device()), what);
+    r.form(g, kind, stream_on(g.device), what);
     return r.value;
 }
 
@@ -166,19 +170,17 @@ Tensor clip_grad_norm(const std::vector<Tensor>& params, double max_norm, double
     const Grads g = collect(params, what);
     check_disjoint(g, what);
     if (g.own.empty()) return torch::zeros({});
-    c10::DeviceGuard guard(g.own[0].device());
+    c10::DeviceGuard guard(g.device);
     if (error_if_nonfinite) check_may_wait(what);
-    void* st = stream_on(g.own[0].device());
+    void* st = stream_on(g.device);
     Norm r(g);
     if (error_if_nonfinite) r.look(g, kind, st, what);
     check_rc(gso_clip_grads(g.n(), g.ptr.data(), g.numel.data(), g.type.data(), kind, max_norm, error_if_nonfinite,
                             r.temp.data_ptr(), r.bytes, r.out(), st),
              what);
     torch::NoGradGuard no_grad;
-    for (size_t i = 0; i < g.own.size(); ++i) {
-        if (!g.packed[i].is_same(g.own[i])) g.own[i].copy_(g.packed[i]);
-        else changed(g.own[i]);
-    }
+    for (const Tensor* t : g.own) changed(*t);
+    for (const auto& copy : g.packed) g.own[copy.first]->copy_(copy.second);
     return r.value;
 }
 
@@ -198,7 +200,7 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
                     scalars.size() == 4 * n && idle.size() == n, what, ": inconsistent lists");
     if (n == 0) return torch::zeros({});
     torch::NoGradGuard no_grad;
-    const c10::Device dev = g.own[0].device();
+    const c10::Device dev = g.device;
     c10::DeviceGuard guard(dev);
     TORCH_CHECK(!capturing(), what, " cannot be captured into a graph: its bias correction follows the step count, which lives "
                 "on the host");
@@ -219,7 +221,7 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
             TORCH_CHECK(t->device() == dev && t->scalar_type() == torch::kFloat32 && t->is_contiguous() &&
                             t->sizes() == p.sizes(), what,
                         ": parameters and moments must be contiguous float32 tensors of one shape on the gradients' device");
-        TORCH_CHECK(g.own[i].scalar_type() == torch::kFloat32, what, ": gradients must be float32");
+        TORCH_CHECK(g.own[i]->scalar_type() == torch::kFloat32, what, ": gradients must be float32");
         TORCH_CHECK(steps[i].numel() == 1, what, ": a step count must be one number");
         if (idle[i]) continue;
         const int64_t rows = p.dim() > 0 ? p.size(0) : 1;
@@ -238,7 +240,7 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
         if (p.numel() == 0) continue;
         TORCH_CHECK(!p.is_neg() && !exp_avg[i].is_neg() && !exp_avg_sq[i].is_neg(), what, ": parameters and moments must hold "
                     "their own values");
-        keep.push_back(plain(g.own[i]).contiguous());
+        keep.push_back(plain(*g.own[i]).contiguous());
         a.param = p.data_ptr<float>();
         a.grad = keep.back().data_ptr<float>();
         a.exp_avg = exp_avg[i].data_ptr<float>();
