@@ -397,21 +397,21 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_write_kernel(int64_t N,
 #pragma unroll
                 for (int j = 0; j < 4; ++j) b[x].above[j] |= all_level ? b[x].level[j] : 0ull;
                 uint32_t at = out + count_below(b[x].above);
-                const int32_t i = (int32_t)((segment + x) * SEGMENT) + 4 * (int)(threadIdx.x & (WAVE - 1));
+                const uint32_t i = (uint32_t)((segment + x) * SEGMENT) + 4 * (threadIdx.x & (WAVE - 1));
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (lane_bit(b[x].above[j])) s_rows[at++] = i + j;
+                    if (lane_bit(b[x].above[j])) s_rows[at++] = (int32_t)(i + j);
                 out += count_rows(b[x].above);
             }
         } else {
 #pragma unroll
             for (int x = 0; x < WAVE_SEGMENTS; ++x) {
                 uint32_t n = pa + count_below(b[x].above), l = pl + count_below(b[x].level);
-                const int32_t i = (int32_t)((segment + x) * SEGMENT) + 4 * (int)(threadIdx.x & (WAVE - 1));
+                const uint32_t i = (uint32_t)((segment + x) * SEGMENT) + 4 * (threadIdx.x & (WAVE - 1));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const bool is_above = lane_bit(b[x].above[j]), is_level = lane_bit(b[x].level[j]);
-                    if (is_above || (is_level && l < need)) s_rows[skip + n + (l < need ? l : need) - level_at] = i + j;
+                    if (is_above || (is_level && l < need)) s_rows[skip + n + (l < need ? l : need) - level_at] = (int32_t)(i + j);
                     n += is_above ? 1u : 0u;
                     l += is_level ? 1u : 0u;
                 }

@@ -126,6 +126,43 @@ def test_selection_of_a_large_model():
         assert np.array_equal(rows.cpu().numpy(), _reference(w, 2_000_000, 100_000))
 
 
+@pytest.mark.parametrize("kind", ["random", "equal", "zeros", "few_values", "near", "special"])
+@pytest.mark.parametrize("N,offset", [(2_200_003, 1), (2_097_153, 0), (9_000_001, 0)])
+def test_selection_in_several_steps_and_tiles(kind, N, offset):
+    """More rows than the workgroups take at once: several loads a thread, several tiles a workgroup."""
+    import gsplat_optim as G
+    gen = torch.Generator(device="cuda").manual_seed(N)
+    w = torch.empty(N + offset, device="cuda")[offset:]
+    w.copy_(_weights(kind, N, gen))
+    for budget, recent in ((N - 1, 0), (N // 3, N // 5 + 1), (17, 3)):
+        rows, _ = G.evict_rows(w, budget, recent)
+        # the same order on the GPU: NaN last, then larger weights, then lower rows (two stable sorts)
+        old = N - recent
+        v = w[:old] + 0.0
+        order = torch.sort(torch.where(v.isnan(), -math.inf, v), descending=True, stable=True).indices
+        order = order[torch.sort(v[order].isnan().to(torch.uint8), stable=True).indices]
+        want = torch.cat((order[:budget - recent].sort().values, torch.arange(old, N, device="cuda"))).to(torch.int32)
+        assert torch.equal(rows, want), (budget, recent)
+
+
+def test_selection_of_the_largest_list():
+    """2^31 - 1 rows: byte offsets beyond 32 bits in weights and rows."""
+    import gsplat_optim as G
+    N = (1 << 31) - 1
+    w = torch.zeros(N, device="cuda")
+    at = [5, 1 << 30, (1 << 30) + 7, N - 260, N - 1]
+    w[at] = torch.tensor([3.0, 2.0, -1.0, -2.0, 1.0], device="cuda")
+    assert G.evict_rows(w, 3)[0].tolist() == [5, 1 << 30, N - 1]
+    assert G.evict_rows(w, 4, 2)[0].tolist() == [5, 1 << 30, N - 2, N - 1]
+    rows = G.evict_rows(w, N - 2)[0]
+    a, b = at[2], at[3]
+    assert rows.shape == (N - 2,)
+    assert rows[[0, a - 1, a, b - 2, b - 1, N - 3]].tolist() == [0, a - 1, a + 1, b - 1, b + 1, N - 1]
+    assert int((rows[1:] - rows[:-1]).max()) == 2 and int((rows[1:] - rows[:-1]).min()) == 1
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        G.evict_rows(torch.zeros(1, device="cuda").expand(1 << 31).contiguous(), 5)
+
+
 def test_selection_takes_a_column_and_any_address():
     import gsplat_optim as G
     base = torch.randn(5003, device="cuda")

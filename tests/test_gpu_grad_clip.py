@@ -514,3 +514,38 @@ def test_lazy_negatives_count_as_what_they_stand_for():
     assert torch.equal(a.clipped_step(1.0), b.clipped_step(1.0)) and torch.equal(want, lazy)
     n = float(G.clip_grad_norm_(lazy, 0.5))
     assert torch.allclose(g, want.grad * (0.5 / (n + 1e-6)), rtol=1e-6)
+
+
+@pytest.mark.parametrize("norm_type", [2.0, 1.0, math.inf])
+def test_gradients_of_many_chunks(norm_type):
+    """Several chunks a workgroup, and a tensor's border inside a round."""
+    import gsplat_optim as G
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    grads = [torch.randn(n, device="cuda", generator=gen).to(t) for n, t in
+             ((20_000_003, torch.float32), (5, torch.float16), (9_000_001, torch.bfloat16), (1, torch.float32))]
+    wide = [g.double() for g in grads]
+    ref = float(torch.linalg.vector_norm(torch.stack([torch.linalg.vector_norm(g, norm_type) for g in wide]), norm_type))
+    n = sum(g.numel() for g in grads)
+    params = _params(grads)
+    got = G.grad_norm(params, norm_type)
+    assert abs(float(got) - ref) <= ref * (U + 8 * n * 2.0 ** -53)
+    assert torch.equal(G.clip_grad_norm_(params, 0.4 * ref, norm_type), got)
+    c = 0.4 * ref / (ref + 1e-6)
+    for g, w in zip(grads, wide):
+        want = w * c
+        assert bool(((g.double() - want).abs() <= want.abs() * (HALF_STEP[g.dtype] + 3 * U) + SUBNORMAL[g.dtype]).all())
+
+
+@pytest.mark.parametrize("N", [9000, 60_000, 125_000])
+@pytest.mark.parametrize("sparse", [None, 0.2])
+def test_clipped_step_of_many_chunks_is_clip_then_step(N, sparse):
+    """Sums joined by the update itself (up to 2048 of them in a sparse step), and by a launch of their own."""
+    import gsplat_optim as G
+    a, b = (_optimizer(N, G.FusedGaussianAdam, steps=1) for _ in range(2))
+    vis = None if sparse is None else torch.rand(N, device="cuda", generator=torch.Generator(device="cuda").manual_seed(N)) < sparse
+    n1 = G.clip_grad_norm_([g["params"][0] for g in b.param_groups], 0.01)
+    b.step(vis, None if vis is None else N)
+    n2 = a.clipped_step(0.01, vis, None if vis is None else N)
+    assert torch.equal(n1, n2)
+    for x, y in zip(_dump(a), _dump(b)):
+        assert torch.equal(x, y)
