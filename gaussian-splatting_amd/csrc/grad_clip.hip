@@ -612,7 +612,8 @@ static hipError_t launch_norm_for(NormUse use, int n, const void* const* grads, 
     });
     if (e != hipSuccess) return e;
     *scaled = small && use == NORM_CLIP;
-    const bool join_later = use != NORM_ONLY && count > 0 && count <= NORM_GROUPS && consumers <= JOIN_CONSUMERS;
+    // without a consumer (a sparse step that no group takes) nobody would join
+    const bool join_later = use != NORM_ONLY && count > 0 && count <= NORM_GROUPS && consumers > 0 && consumers <= JOIN_CONSUMERS;
     if (!small && !join_later) {
         if (kind == 2) launch_finish<2>(norm_partials(temp), count, max_norm, r, norm, st);
         else if (kind == 1) launch_finish<1>(norm_partials(temp), count, max_norm, r, norm, st);

@@ -549,3 +549,21 @@ def test_clipped_step_of_many_chunks_is_clip_then_step(N, sparse):
     assert torch.equal(n1, n2)
     for x, y in zip(_dump(a), _dump(b)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("n", [10, 40_000, 1_000_000])
+def test_a_step_that_no_group_takes_still_returns_the_norm(n):
+    """A sparse step whose N no group has: the norm counts all gradients, and nothing moves."""
+    import gsplat_optim as G
+    p = torch.nn.Parameter(torch.ones(n, 3, device="cuda"))
+    p.grad = torch.full((n, 3), 2.0, device="cuda")
+    opt = G.FusedGaussianAdam([p], lr=0.1)
+    vis = torch.ones(7, dtype=torch.bool, device="cuda")
+    poison = torch.full((1 << 20,), math.nan, device="cuda")     # what a fresh allocation may hold
+    del poison
+    for _ in range(2):
+        assert float(opt.clipped_step(1.0, vis, 7)) == pytest.approx(2.0 * math.sqrt(3 * n), rel=1e-6)
+    assert bool((p == 1).all())
+    empty = torch.nn.Parameter(torch.ones(0, 3, device="cuda"))
+    empty.grad = torch.ones(0, 3, device="cuda")
+    assert float(G.FusedGaussianAdam([empty], lr=0.1).clipped_step(1.0)) == 0.0
