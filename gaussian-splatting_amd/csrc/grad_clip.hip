@@ -583,9 +583,9 @@ static void launch_finish(const uint64_t* p, int count, double max_norm, NormRes
     hipLaunchKernelGGL(norm_finish_kernel<KIND>, dim3(1), dim3(FINISH_THREADS), 0, st, p, count, max_norm, r, norm);
 }
 
-// The norm of the gradients for whoever reads it next.  FINISH: the result in the temp area and in *norm; otherwise
-// *c says where the coefficient is found.  A clip of a few chunks is done at once (*scaled).  `consumers`: workgroups of
-// what reads the coefficient.
+// The norm of the gradients for whoever reads it next: *c says where the coefficient is found; for a norm alone the
+// result is in the temp area and in *norm.  A clip of a few chunks is done at once (*scaled).  `consumers`: workgroups
+// of what reads the coefficient.
 constexpr uint32_t SMALL_CHUNKS = 16;
 constexpr int64_t JOIN_CONSUMERS = 1024;   // clip of 10 MB: 9.5 us with, 11.2 without; of 25 MB (1539): 16.9 and 15.5
 enum NormUse { NORM_ONLY, NORM_CLIP, NORM_STEP };
