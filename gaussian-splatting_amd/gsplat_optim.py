@@ -127,7 +127,6 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     return _host().clip_grad_norm(_tensors(parameters), float(max_norm), float(norm_type), bool(error_if_nonfinite))
 
 
-@torch.no_grad()
 def clipped_adam_step(optimizer, max_norm, visibility=None, N=None, norm_type=2.0, error_if_nonfinite=False):
     """`clip_grad_norm_(all parameters of the optimizer, max_norm)` followed by `FusedGaussianAdam.step(visibility, N)`
     for a torch.optim.Adam (or FusedGaussianAdam): one pass that sums and one that updates every tensor, which
@@ -144,36 +143,32 @@ def clipped_adam_step(optimizer, max_norm, visibility=None, N=None, norm_type=2.
         raise RuntimeError(f"{what} needs a torch.optim.Adam, got {type(optimizer).__name__}")
     if not float(max_norm) >= 0.0:
         raise RuntimeError(f"{what}: max_norm must not be negative or NaN, got {max_norm}")
-    entries = []
     for group in optimizer.param_groups:
-        if any(group.get(k) for k in ("weight_decay", "amsgrad", "maximize", "capturable", "differentiable", "fused")):
+        if group["weight_decay"] or group["amsgrad"] or group["maximize"] or group["capturable"] or \
+                group["differentiable"] or group["fused"]:
             raise RuntimeError(f"{what}: weight_decay, amsgrad, maximize, capturable, differentiable and fused are not supported")
-        beta1, beta2 = group["betas"]
-        scalars = (float(group["lr"]), float(beta1), float(beta2), float(group["eps"]))
-        for p in group["params"]:
-            if p.grad is None:
-                continue
-            if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
-                raise RuntimeError(f"{what} needs contiguous float32 GPU parameters (there is no CPU path)")
-            # a group that is not per-Gaussian takes no sparse step
-            idle = visibility is not None and N is not None and (p.shape[0] if p.dim() > 0 else 1) != N
-            entries.append((p, scalars, idle))
-    params, m, v, steps, flat, idles, fresh = [], [], [], [], [], [], []
+    by_rows = visibility is not None and N is not None   # then a group that is not per-Gaussian takes no step
+    params, m, v, steps, scalars, idle, fresh = [], [], [], [], [], [], []
     try:
-        for p, scalars, idle in entries:
-            st = optimizer.state[p]
-            if len(st) == 0:
-                fresh.append(p)
-                st["step"] = torch.tensor(0.0, dtype=torch.float32)
-                st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            params.append(p)
-            m.append(st["exp_avg"])
-            v.append(st["exp_avg_sq"])
-            steps.append(st["step"])
-            flat += scalars
-            idles.append(idle)
-        return _host().clipped_adam(params, m, v, steps, flat, idles, visibility, float(max_norm), float(norm_type),
+        for group in optimizer.param_groups:
+            beta1, beta2 = group["betas"]
+            numbers = (float(group["lr"]), float(beta1), float(beta2), float(group["eps"]))
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                st = optimizer.state[p]
+                if len(st) == 0:
+                    fresh.append(p)
+                    st["step"] = torch.tensor(0.0, dtype=torch.float32)
+                    st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                    st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                params.append(p)
+                m.append(st["exp_avg"])
+                v.append(st["exp_avg_sq"])
+                steps.append(st["step"])
+                scalars += numbers
+                idle.append(by_rows and (p.shape[0] if p.dim() > 0 else 1) != N)
+        return _host().clipped_adam(params, m, v, steps, scalars, idle, visibility, float(max_norm), float(norm_type),
                                     bool(error_if_nonfinite))
     except Exception:
         for p in fresh:
