@@ -194,10 +194,17 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
                     double max_norm, double norm_type, bool error_if_nonfinite) {
     const char* what = "clipped_adam_step";
     const int kind = norm_kind(norm_type, what);
-    const Grads g = collect(params, what);
     const size_t n = params.size();
-    TORCH_CHECK(g.own.size() == n && exp_avg.size() == n && exp_avg_sq.size() == n && steps.size() == n &&
-                    scalars.size() == 4 * n && idle.size() == n, what, ": inconsistent lists");
+    TORCH_CHECK(exp_avg.size() == n && exp_avg_sq.size() == n && steps.size() == n && scalars.size() == 4 * n &&
+                    idle.size() == n, what, ": inconsistent lists");
+    // A gradient outlives `parameter.data = other`: the update would read as many elements as the parameter now has.
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor& grad = params[i].grad();
+        TORCH_CHECK(idle[i] || !grad.defined() || grad.sizes() == params[i].sizes(), what, ": a gradient of shape ",
+                    grad.sizes(), " does not have its parameter's shape ", params[i].sizes());
+    }
+    const Grads g = collect(params, what);
+    TORCH_CHECK(g.own.size() == n, what, ": inconsistent lists");
     if (n == 0) return torch::zeros({});
     torch::NoGradGuard no_grad;
     const c10::Device dev = g.device;

@@ -60,6 +60,25 @@ def test_arguments_are_checked_before_anything_runs():
     assert float(G.grad_norm([])) == 0.0 and float(G.clip_grad_norm_([torch.nn.Parameter(torch.ones(2))], 1.0)) == 0.0
 
 
+def _stale(device="cpu", rows=8):
+    """A parameter that was given more rows while its gradient kept the old ones."""
+    p = torch.nn.Parameter(torch.ones(4, 3, device=device))
+    p.grad = torch.ones(4, 3, device=device)
+    p.data = torch.ones(rows, 3, device=device)
+    assert p.grad.shape == (4, 3)
+    return p
+
+
+def test_a_gradient_of_another_shape_is_refused_by_the_clipped_step():
+    import gsplat_optim as G
+    for rows in (8, 3, 0):
+        p = _stale(rows=rows)
+        opt = torch.optim.Adam([p])
+        with pytest.raises(RuntimeError, match="does not have its parameter's shape"):
+            G.clipped_adam_step(opt, 1.0)
+        assert len(opt.state) == 0 and torch.equal(p.detach(), torch.ones(rows, 3))
+
+
 def test_c_abi_refuses_bad_arguments():
     from _gsplat_lib import lib
     L = lib()

@@ -567,3 +567,26 @@ def test_a_step_that_no_group_takes_still_returns_the_norm(n):
     empty = torch.nn.Parameter(torch.ones(0, 3, device="cuda"))
     empty.grad = torch.ones(0, 3, device="cuda")
     assert float(G.FusedGaussianAdam([empty], lr=0.1).clipped_step(1.0)) == 0.0
+
+
+def test_a_gradient_of_another_shape_is_refused():
+    """`parameter.data = other` leaves the old gradient behind; the update would read past its end."""
+    import gsplat_optim as G
+    p = torch.nn.Parameter(torch.ones(100, 3, device="cuda"))
+    q = torch.nn.Parameter(torch.ones(50, device="cuda"))
+    opt = G.FusedGaussianAdam([{"params": [p]}, {"params": [q]}], lr=0.1)
+    for t in (p, q):
+        t.grad = torch.full_like(t, 0.5)
+    opt.clipped_step(1.0)
+    state = {k: {n: x.clone() for n, x in opt.state[k].items()} for k in (p, q)}
+    for shape in ((200, 3), (99, 3), (300,), (100, 3, 1)):
+        p.data = torch.ones(shape, device="cuda")
+        for k in ("exp_avg", "exp_avg_sq"):
+            opt.state[p][k] = torch.ones(shape, device="cuda")
+        before = q.detach().clone()
+        for kw in ({}, dict(error_if_nonfinite=True)):
+            with pytest.raises(RuntimeError, match="does not have its parameter's shape"):
+                opt.clipped_step(1.0, **kw)
+        assert torch.equal(p.detach(), torch.ones(shape, device="cuda")) and torch.equal(q.detach(), before)
+        assert all(torch.equal(opt.state[q][n], x) for n, x in state[q].items()) and float(opt.state[p]["step"]) == 1.0
+        assert all(bool((opt.state[p][n] == 1).all()) for n in ("exp_avg", "exp_avg_sq"))
