@@ -49,6 +49,9 @@ class FusedGaussianAdam(torch.optim.Adam):
             for p in group["params"]:
                 if p.grad is None:
                     continue
+                if p.grad.shape != p.shape:   # a gradient outlives `p.data = other`
+                    raise RuntimeError(f"FusedGaussianAdam: a gradient of shape {tuple(p.grad.shape)} does not have its "
+                                       f"parameter's shape {tuple(p.shape)}")
                 if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
                     raise RuntimeError("FusedGaussianAdam needs contiguous float32 GPU parameters (there is no CPU path)")
                 g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
@@ -57,6 +60,11 @@ class FusedGaussianAdam(torch.optim.Adam):
                     st["step"] = torch.tensor(0.0, dtype=torch.float32)
                     st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                     st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                for t in (g, st["exp_avg"], st["exp_avg_sq"]):
+                    if t.shape != p.shape or t.dtype != torch.float32 or t.device != p.device or not t.is_contiguous():
+                        raise RuntimeError("FusedGaussianAdam: gradient and moments must be contiguous float32 tensors of the "
+                                           f"parameter's shape {tuple(p.shape)} on {p.device}, got {tuple(t.shape)} {t.dtype} "
+                                           f"on {t.device}")
                 rows = p.shape[0] if p.dim() > 0 else 1
                 width = p.numel() // max(rows, 1)
                 if vis is not None:

@@ -79,6 +79,16 @@ def test_a_gradient_of_another_shape_is_refused_by_the_clipped_step():
         assert len(opt.state) == 0 and torch.equal(p.detach(), torch.ones(rows, 3))
 
 
+def test_a_gradient_of_another_shape_is_refused_by_the_step():
+    import gsplat_optim as G
+    for rows in (8, 3, 0):
+        p = _stale(rows=rows)
+        opt = G.FusedGaussianAdam([p])
+        with pytest.raises(RuntimeError, match="does not have its parameter's shape"):
+            opt.step()
+        assert len(opt.state) == 0 and torch.equal(p.detach(), torch.ones(rows, 3))
+
+
 def test_c_abi_refuses_bad_arguments():
     from _gsplat_lib import lib
     L = lib()

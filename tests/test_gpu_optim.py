@@ -338,3 +338,38 @@ def test_mark_nonzero_is_the_or_of_the_counts(P, narrays):
           "gso_mark_nonzero")
     torch.cuda.synchronize()
     assert torch.equal(t, want.to(torch.uint8))
+
+
+def test_a_step_on_tensors_that_do_not_match_is_refused():
+    """The kernel takes as many elements of gradient and moments as the parameter has."""
+    from gsplat_optim import FusedGaussianAdam
+    def make():
+        p = torch.nn.Parameter(torch.ones(100, 3, device="cuda:0"))
+        opt = FusedGaussianAdam([p], lr=0.1)
+        p.grad = torch.full((100, 3), 0.5, device="cuda:0")
+        opt.step()
+        return p, opt
+    p, opt = make()
+    for shape in ((200, 3), (99, 3), (100, 3, 1)):
+        p.data = torch.ones(shape, device="cuda:0")
+        with pytest.raises(RuntimeError, match="does not have its parameter's shape"):
+            opt.step()
+        assert bool((p == 1).all()) and float(opt.state[p]["step"]) == 1.0
+    good = dict(device="cuda:0")
+    for bad in (torch.zeros(99, 3, **good), torch.zeros(100, 4, **good), torch.zeros(100, 3), torch.zeros(100, 3, **good).double(),
+                torch.zeros(3, 100, **good).t()):
+        for key in ("exp_avg", "exp_avg_sq"):
+            p, opt = make()
+            before = p.detach().clone()
+            opt.state[p][key] = bad
+            with pytest.raises(RuntimeError, match="moments must be contiguous float32"):
+                opt.step()
+            assert torch.equal(p.detach(), before) and float(opt.state[p]["step"]) == 1.0
+    # a gradient in another order is still packed first, as before
+    p, opt = make()
+    q, other = make()
+    p.grad = torch.arange(300.0, device="cuda:0").view(3, 100).t()
+    q.grad = p.grad.contiguous()
+    opt.step()
+    other.step()
+    assert torch.equal(p, q)
