@@ -52,6 +52,8 @@ class FusedGaussianAdam(torch.optim.Adam):
                 if p.grad.shape != p.shape:   # a gradient outlives `p.data = other`
                     raise RuntimeError(f"FusedGaussianAdam: a gradient of shape {tuple(p.grad.shape)} does not have its "
                                        f"parameter's shape {tuple(p.shape)}")
+                if vis is not None and vis.device != p.device:
+                    raise RuntimeError(f"FusedGaussianAdam: visibility must be on {p.device}, got {vis.device}")
                 if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
                     raise RuntimeError("FusedGaussianAdam needs contiguous float32 GPU parameters (there is no CPU path)")
                 g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()

@@ -89,6 +89,15 @@ def test_a_gradient_of_another_shape_is_refused_by_the_step():
         assert len(opt.state) == 0 and torch.equal(p.detach(), torch.ones(rows, 3))
 
 
+def test_visibility_of_another_device_is_refused_by_the_step():
+    import gsplat_optim as G
+    p = _param()
+    opt = G.FusedGaussianAdam([p])
+    with pytest.raises(RuntimeError, match="visibility must be on cpu, got meta"):
+        opt.step(torch.ones(4, dtype=torch.bool, device="meta"), 4)
+    assert len(opt.state) == 0 and torch.equal(p.detach(), torch.ones(4, 3))
+
+
 def test_c_abi_refuses_bad_arguments():
     from _gsplat_lib import lib
     L = lib()

@@ -373,3 +373,16 @@ def test_a_step_on_tensors_that_do_not_match_is_refused():
     opt.step()
     other.step()
     assert torch.equal(p, q)
+
+
+def test_a_sparse_step_with_visibility_in_host_memory_is_refused():
+    from gsplat_optim import FusedGaussianAdam
+    p = torch.nn.Parameter(torch.ones(100, 3, device="cuda:0"))
+    p.grad = torch.ones_like(p)
+    opt = FusedGaussianAdam([p], lr=0.1)
+    for vis in (torch.ones(100, dtype=torch.bool), torch.ones(100, dtype=torch.uint8)):
+        with pytest.raises(RuntimeError, match="visibility must be on cuda:0, got cpu"):
+            opt.step(vis, 100)
+    assert len(opt.state) == 0 and bool((p == 1).all())
+    opt.step(torch.ones(100, dtype=torch.bool, device="cuda:0"), 100)
+    assert bool((p < 1).all())
