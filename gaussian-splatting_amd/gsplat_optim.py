@@ -41,8 +41,9 @@ class FusedGaussianAdam(torch.optim.Adam):
         L = lib()
         vis = None
         if visibility is not None:
-            vis = visibility.to(torch.uint8) if visibility.dtype != torch.uint8 else visibility
-            vis = vis.contiguous()
+            # a row is visible where the mask is not zero, whatever its type (radii, weights)
+            vis = visibility if visibility.dtype in (torch.bool, torch.uint8) else visibility != 0
+            vis = vis.contiguous().view(torch.uint8)
         for group in self.param_groups:
             beta1, beta2 = group["betas"]
             lr, eps = float(group["lr"]), float(group["eps"])

@@ -590,3 +590,24 @@ def test_a_gradient_of_another_shape_is_refused():
         assert torch.equal(p.detach(), torch.ones(shape, device="cuda")) and torch.equal(q.detach(), before)
         assert all(torch.equal(opt.state[q][n], x) for n, x in state[q].items()) and float(opt.state[p]["step"]) == 1.0
         assert all(bool((opt.state[p][n] == 1).all()) for n in ("exp_avg", "exp_avg_sq"))
+
+
+@pytest.mark.parametrize("make", [
+    lambda on: on.to(torch.int32) * 256, lambda on: on.to(torch.int64) << 40, lambda on: on.float() * 0.5, lambda on: on.half() * -0.25,
+    lambda on: on.to(torch.int16) * -512, lambda on: on.to(torch.int8) * -128, lambda on: on.to(torch.uint8) * 200, lambda on: on,
+    lambda on: on.double()[:, None] * 1e-300, lambda on: torch.stack((on, ~on), 1)[:, 0]])
+def test_a_row_is_visible_where_the_mask_is_not_zero(make):
+    """In both steps, whatever the mask's type: radii and weights serve as masks as they are."""
+    N = 3001
+    on = torch.rand(N, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) < 0.4
+    import gsplat_optim as G
+    a, b, c = (_optimizer(N, G.FusedGaussianAdam) for _ in range(3))
+    before = _dump(a)
+    mask = make(on)
+    a.step(on, N)
+    b.step(mask, N)
+    c.clipped_step(1e30, mask, N)
+    for x, y, z, was in zip(_dump(a), _dump(b), _dump(c), before):
+        assert torch.equal(x, y) and torch.equal(x, z)
+        if x.dim() > 0:
+            assert torch.equal(x[~on], was[~on])
