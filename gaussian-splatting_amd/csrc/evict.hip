@@ -592,12 +592,16 @@ __device__ __forceinline__ void copy_narrow(const RowRun& s, T* __restrict__ dst
     constexpr uint32_t N = 16 / sizeof(T);
     const bool dense = s.pitch == (int64_t)(s.M * sizeof(T));
     for (uint32_t q = threadIdx.x; q < vectors; q += 256) {
-        const uint32_t x = q * N, r0 = s.row(x), c0 = x - r0 * s.M;
+        const uint32_t x = q * N, c0 = x - s.row(x) * s.M;
         int32_t at[N];
 #pragma unroll
         for (uint32_t j = 0; j < N; ++j) at[j] = s.rows[s.row(x + j)];
         f32x4 v;
-        if (dense && at[N - 1] - at[0] == (int32_t)(s.row(x + N - 1) - r0)) {   // rows ascend
+        // rows that follow each other, each one: repeated and unordered rows can span as much as a run does
+        bool run = dense;
+#pragma unroll
+        for (uint32_t j = 1; j < N; ++j) run = run && at[j] - at[j - 1] == (int32_t)(s.row(x + j) - s.row(x + j - 1));
+        if (run) {
             v = *reinterpret_cast<const vector_of<T>*>(s.src + (int64_t)at[0] * s.pitch + c0 * sizeof(T));
         } else {
             union { f32x4 v; T t[N]; } e;

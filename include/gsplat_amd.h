@@ -495,7 +495,7 @@ int gso_adam_clipped(int ngrads, const void* const* grads, const int64_t* numels
  *     kept, -0 equals 0, and a NaN lies below everything.  0 <= recent <= budget, N < 2^31.
  *     temp: device, gso_evict_temp_bytes(N).
  *   gso_gather_rows_multi: for each of n tensors dst[r] = src[rows[r]], r < K: rows of row_bytes bytes of any type,
- *     src_pitch bytes apart in src and packed in dst.  Entries of `rows` must lie in every src and ascend.
+ *     src_pitch bytes apart in src and packed in dst.  Entries of `rows` must lie in every src; any order, also repeated.
  * None waits for the device: the number of kept rows is known beforehand. */
 typedef struct {
     const void* src;

@@ -442,3 +442,32 @@ def test_lazy_conjugates_and_a_single_tensor():
     acc = torch.zeros(100, device="cuda")
     G.accumulate_weights(acc, [lazy])
     assert torch.equal(acc, w)
+
+
+@pytest.mark.parametrize("row_bytes,pitch", [(1, 1), (2, 2), (4, 4), (8, 8), (3, 3), (6, 6), (12, 12), (16, 16), (180, 180), (4, 12), (1, 0)])
+@pytest.mark.parametrize("order", ["repeats", "descending", "random", "pairs"])
+def test_c_abi_copies_rows_in_any_order(row_bytes, pitch, order):
+    """Repeated and unordered rows: a vector of the copy whose first and last row are as far apart as in a run of rows
+    need not be one."""
+    import ctypes as C
+    from _gsplat_lib import check, lib
+    N, K = 500, 1003
+    gen = torch.Generator(device="cuda").manual_seed(row_bytes)
+    src = torch.randint(0, 250, (N * max(pitch, row_bytes),), device="cuda", generator=gen, dtype=torch.int32).to(torch.uint8)
+    dst = torch.full((K * row_bytes,), 255, dtype=torch.uint8, device="cuda")
+    if order == "repeats":      # 5 5 7 8, 9 9 11 12, ...: ascending, the span of a run
+        rows = (torch.arange(K, device="cuda") + 5 - (torch.arange(K, device="cuda") % 4 == 1).long()) % (N - 8)
+    elif order == "descending":
+        rows = torch.arange(K, device="cuda").flip(0) % N
+    elif order == "random":
+        rows = torch.randint(0, N, (K,), device="cuda", generator=gen)
+    else:                       # 0 2 1 3, 4 6 5 7, ...
+        k = torch.arange(K, device="cuda")
+        rows = (k + (k % 4 == 1).long() - (k % 4 == 2).long()) % (N - 8)
+    rows = rows.to(torch.int32)
+    assert int(rows.min()) >= 0 and int(rows.max()) < N
+    entry = (C.c_int64 * 4)(src.data_ptr(), dst.data_ptr(), row_bytes, pitch)
+    check(lib().gso_gather_rows_multi(1, C.addressof(entry), rows.data_ptr(), K, torch.cuda.current_stream().cuda_stream), "gather")
+    at = rows.long()[:, None] * pitch + torch.arange(row_bytes, device="cuda")[None]
+    torch.cuda.synchronize()
+    assert torch.equal(dst.view(K, row_bytes), src[at])
