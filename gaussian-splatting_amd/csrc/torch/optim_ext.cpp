@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <functional>
 #include <vector>
 
 #include "../../../include/gsplat_amd.h"
@@ -110,18 +111,108 @@ Grads collect(const std::vector<Tensor>& params, const char* what) {
     return g;
 }
 
-// Scaling in place needs every element once: two gradients in the same memory would race.
-void check_disjoint(const Grads& g, const char* what) {
-    for (const auto& copy : g.packed) {
-        const Tensor& t = *g.own[copy.first];
-        for (int64_t d = 0; d < t.dim(); ++d)
-            TORCH_CHECK(t.stride(d) != 0 || t.size(d) <= 1, what,
-                        ": a gradient has several elements in one place (an expanded tensor)");
+// Whether x_0 * stride_0 + x_1 * stride_1 + ... = target has a solution in 0 <= x_k <= most_k.  Larger strides first; in the
+// layouts of tensors each leaves the next a few values.  A search that takes too long counts as a solution.
+struct Places {
+    std::vector<std::pair<int64_t, int64_t>> terms;   // (stride > 0, most > 0)
+    void add(int64_t stride, int64_t most) {
+        if (most <= 0) return;
+        for (auto& t : terms)
+            if (t.first == stride) {
+                t.second += most;
+                return;
+            }
+        terms.emplace_back(stride, most);
     }
-    Spans spans;
-    spans.all.reserve(g.own.size());
-    for (size_t i = 0; i < g.own.size(); ++i) spans.add(g.ptr[i], g.numel[i] * (g.type[i] == GSO_F32 ? 4 : 2), true);
-    TORCH_CHECK(spans.disjoint(), what, ": two gradients share memory (is a parameter listed twice?)");
+    bool reach(int64_t target) {
+        std::sort(terms.begin(), terms.end(), std::greater<>());
+        int64_t rest = 0;
+        for (const auto& t : terms) rest += t.first * t.second;
+        int64_t steps = 1 << 20;
+        return search(0, target, rest, steps);
+    }
+    bool search(size_t k, int64_t target, int64_t rest, int64_t& steps) const {   // rest: the most that terms k and on can give
+        if (target < 0 || target > rest) return false;
+        if (target == 0 || --steps <= 0) return true;
+        const int64_t stride = terms[k].first, after = rest - stride * terms[k].second;
+        const int64_t low = target > after ? (target - after + stride - 1) / stride : 0;
+        for (int64_t x = std::min(terms[k].second, target / stride); x >= low; --x)
+            if (search(k + 1, target - x * stride, after, steps)) return true;
+        return false;
+    }
+};
+
+// Bytes from a tensor's first element to its last one.
+int64_t bytes_to_last(const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return last * t.element_size();
+}
+
+// The tensor's bytes as a sum: element, and one term per dimension.
+void add_bytes(Places& p, const Tensor& t) {
+    if (t.is_non_overlapping_and_dense()) {
+        p.add(1, t.numel() * t.element_size() - 1);
+        return;
+    }
+    p.add(1, t.element_size() - 1);
+    for (int64_t d = 0; d < t.dim(); ++d) p.add(t.stride(d) * t.element_size(), t.size(d) - 1);
+}
+
+// Byte i of a is byte j of b: with j counted from b's end all terms are positive.
+bool share_bytes(const Tensor& a, const Tensor& b) {
+    Places p;
+    add_bytes(p, a);
+    add_bytes(p, b);
+    return p.reach((int64_t)((uintptr_t)b.data_ptr() - (uintptr_t)a.data_ptr()) + bytes_to_last(b) + b.element_size() - 1);
+}
+
+// Two indices of a tensor at one place: in the dimension of largest stride in which they differ they differ by x + 1, in those
+// of smaller strides by anything, d_q = y_q - (size_q - 1).
+bool meets_itself(const Tensor& t) {
+    if (t.is_non_overlapping_and_dense()) return false;
+    std::vector<std::pair<int64_t, int64_t>> dims;   // (stride, size - 1)
+    for (int64_t d = 0; d < t.dim(); ++d) {
+        if (t.size(d) <= 1) continue;
+        if (t.stride(d) == 0) return true;
+        dims.emplace_back(t.stride(d), t.size(d) - 1);
+    }
+    std::sort(dims.begin(), dims.end());
+    for (size_t k = 0; k < dims.size(); ++k) {
+        Places p;
+        int64_t target = -dims[k].first;
+        p.add(dims[k].first, dims[k].second - 1);
+        for (size_t q = 0; q < k; ++q) {
+            p.add(dims[q].first, 2 * dims[q].second);
+            target += dims[q].first * dims[q].second;
+        }
+        if (p.reach(target)) return true;
+    }
+    return false;
+}
+
+// Scaling in place needs every element once: two gradients in the same memory would race, or count twice in the norm.
+// Slices of one buffer may lie between each other.
+void check_disjoint(const std::vector<Tensor>& params, const char* what) {
+    struct Span {
+        uintptr_t begin, end;
+        const Tensor* t;
+    };
+    std::vector<Span> all;
+    all.reserve(params.size());
+    for (const Tensor& p : params) {
+        if (!p.defined()) continue;
+        const Tensor& t = p.grad();
+        if (!t.defined() || t.layout() != c10::kStrided || t.numel() == 0) continue;
+        TORCH_CHECK(!meets_itself(t), what, ": a gradient has several elements in one place (an expanded tensor)");
+        const uintptr_t begin = (uintptr_t)t.data_ptr();
+        all.push_back({begin, begin + (uintptr_t)(bytes_to_last(t) + t.element_size()), &t});
+    }
+    const auto before = [](const Span& a, const Span& b) { return a.begin < b.begin; };
+    if (!std::is_sorted(all.begin(), all.end(), before)) std::sort(all.begin(), all.end(), before);
+    for (size_t i = 0; i < all.size(); ++i)
+        for (size_t j = i + 1; j < all.size() && all[j].begin < all[i].end; ++j)
+            TORCH_CHECK(!share_bytes(*all[i].t, *all[j].t), what, ": two gradients share memory (is a parameter listed twice?)");
 }
 
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
@@ -167,8 +258,8 @@ Tensor clip_grad_norm(const std::vector<Tensor>& params, double max_norm, double
     const char* what = "clip_grad_norm_";
     const int kind = norm_kind(norm_type, what);
     TORCH_CHECK(max_norm >= 0.0, what, ": max_norm must not be negative or NaN, got ", max_norm);
+    check_disjoint(params, what);
     const Grads g = collect(params, what);
-    check_disjoint(g, what);
     if (g.own.empty()) return torch::zeros({});
     c10::DeviceGuard guard(g.device);
     if (error_if_nonfinite) check_may_wait(what);

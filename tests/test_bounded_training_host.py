@@ -98,6 +98,64 @@ def test_visibility_of_another_device_is_refused_by_the_step():
     assert len(opt.state) == 0 and torch.equal(p.detach(), torch.ones(4, 3))
 
 
+def _with_grads(*grads):
+    out = []
+    for g in grads:
+        p = torch.nn.Parameter(torch.empty(g.shape, dtype=g.dtype))
+        p.grad = g
+        out.append(p)
+    return out
+
+
+def test_strided_gradients_that_share_memory_are_refused():
+    import gsplat_optim as G
+    wide = torch.zeros(50, 8)
+    other = wide.view(torch.bfloat16)
+    for grads in ((wide[:, 2:5], wide[:, 4:6]), (wide[:, 1], wide), (wide, wide[::2, ::2]), (wide[::2], wide[4]), (wide[:, :3], wide[:, :3]),
+                  (wide[:, 0], other[:, 1]), (wide[:, 0], wide[:, 1], other[:, 3]), (wide.t()[3:5], wide[:, 4:])):
+        with pytest.raises(RuntimeError, match="share memory"):
+            G.clip_grad_norm_(_with_grads(*grads), 1.0)
+    for grads in ((wide[:, :3], wide[:, 3:5], wide[:, 5:]), (wide[::2], wide[1::2]), (wide[:, ::2], wide[:, 1::2]), (wide[:, 0], other[:, 2::3]),
+                  (wide[:25, 1:].t(), wide[25:]), tuple(wide[:, k] for k in range(8))):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            G.clip_grad_norm_(_with_grads(*grads), 1.0)
+    line = torch.zeros(100)
+    for size, stride in (((5, 3), (1, 1)), ((4, 2), (2, 4)), ((5,), (0,)), ((3, 3, 3), (9, 2, 4))):
+        with pytest.raises(RuntimeError, match="several elements in one place"):
+            G.clip_grad_norm_(_with_grads(line.as_strided(size, stride)), 1.0)
+    for size, stride in (((3, 2), (2, 3)), ((5, 1), (2, 0)), ((4, 4), (10, 2))):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            G.clip_grad_norm_(_with_grads(line.as_strided(size, stride)), 1.0)
+
+
+def test_shared_memory_is_found_as_by_listing_every_byte():
+    import random
+
+    import gsplat_optim as G
+    rng = random.Random(11)
+    memory = torch.zeros(4096, dtype=torch.uint8)
+    verdicts = []
+    for _ in range(4000):
+        grads, places = [], []
+        for _ in range(2):
+            dtype = rng.choice([torch.float32, torch.bfloat16, torch.float16])
+            size = [rng.randint(1, 5) for _ in range(rng.randint(1, 3))]
+            stride = [rng.choice([1, 2, 3, 4, 6, 7, 8, 12, 20]) for _ in size]
+            base = memory.view(dtype)
+            t = base.as_strided(size, stride, rng.randint(0, 60))
+            e = t.element_size()
+            places.append([b for i in torch.cartesian_prod(*[torch.arange(n) for n in size]).view(-1, len(size)).tolist()
+                           for b in range(e * (t.storage_offset() + sum(x * s for x, s in zip(i, stride))),
+                                          e * (t.storage_offset() + sum(x * s for x, s in zip(i, stride))) + e)])
+            grads.append(t)
+        alone = any(len(set(p)) < len(p) for p in places)
+        want = "several elements" if alone else "share memory" if set(places[0]) & set(places[1]) else "no CPU path"
+        with pytest.raises(RuntimeError, match=want):
+            G.clip_grad_norm_(_with_grads(*grads), 1.0)
+        verdicts.append(want)
+    assert min(verdicts.count(v) for v in set(verdicts)) > 300 and len(set(verdicts)) == 3
+
+
 def test_c_abi_refuses_bad_arguments():
     from _gsplat_lib import lib
     L = lib()

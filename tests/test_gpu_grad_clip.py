@@ -611,3 +611,22 @@ def test_a_row_is_visible_where_the_mask_is_not_zero(make):
         assert torch.equal(x, y) and torch.equal(x, z)
         if x.dim() > 0:
             assert torch.equal(x[~on], was[~on])
+
+
+def test_strided_gradients_that_share_memory_are_refused():
+    """They are scaled in packed copies; their own memory is what must not be shared."""
+    import gsplat_optim as G
+    wide = torch.randn(50, 8, device="cuda")
+    keep = wide.clone()
+    for grads in ((wide[:, 2:5], wide[:, 4:6]), (wide[:, 1], wide), (wide, wide[::2, ::2]), (wide[:, :3], wide[:, :3])):
+        with pytest.raises(RuntimeError, match="share memory"):
+            G.clip_grad_norm_(_params(grads), 1.0)
+    with pytest.raises(RuntimeError, match="several elements in one place"):
+        G.clip_grad_norm_(_params([wide.view(-1).as_strided((5, 3), (1, 1))]), 1.0)
+    assert torch.equal(wide, keep)
+    columns = [wide[:, :3], wide[:, 3:5], wide[:, 5], wide[:, 6:].t()]      # one buffer, every element once
+    norm = G.clip_grad_norm_(_params(columns), 0.1)
+    ref = _norm64([keep], 2.0)
+    assert abs(float(norm) - ref) <= ref * (U + 1e-11)
+    c = 0.1 / (ref + 1e-6)
+    assert bool(((wide.double() - keep.double() * c).abs() <= keep.double().abs() * c * 3 * U + SUBNORMAL[torch.float32]).all())
