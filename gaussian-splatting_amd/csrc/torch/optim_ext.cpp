@@ -170,7 +170,6 @@ bool share_bytes(const Tensor& a, const Tensor& b) {
 // Two indices of a tensor at one place: in the dimension of largest stride in which they differ they differ by x + 1, in those
 // of smaller strides by anything, d_q = y_q - (size_q - 1).
 bool meets_itself(const Tensor& t) {
-    if (t.is_non_overlapping_and_dense()) return false;
     std::vector<std::pair<int64_t, int64_t>> dims;   // (stride, size - 1)
     for (int64_t d = 0; d < t.dim(); ++d) {
         if (t.size(d) <= 1) continue;
@@ -204,9 +203,10 @@ void check_disjoint(const std::vector<Tensor>& params, const char* what) {
         if (!p.defined()) continue;
         const Tensor& t = p.grad();
         if (!t.defined() || t.layout() != c10::kStrided || t.numel() == 0) continue;
-        TORCH_CHECK(!meets_itself(t), what, ": a gradient has several elements in one place (an expanded tensor)");
+        const bool dense = t.is_non_overlapping_and_dense();
+        TORCH_CHECK(dense || !meets_itself(t), what, ": a gradient has several elements in one place (an expanded tensor)");
         const uintptr_t begin = (uintptr_t)t.data_ptr();
-        all.push_back({begin, begin + (uintptr_t)(bytes_to_last(t) + t.element_size()), &t});
+        all.push_back({begin, begin + (uintptr_t)(dense ? (int64_t)t.nbytes() : bytes_to_last(t) + t.element_size()), &t});
     }
     const auto before = [](const Span& a, const Span& b) { return a.begin < b.begin; };
     if (!std::is_sorted(all.begin(), all.end(), before)) std::sort(all.begin(), all.end(), before);
