@@ -73,6 +73,8 @@ struct Spans {
 // fill a block of memory of their own (a slice of something wider) is worked on in a packed copy.
 struct Grads {
     std::vector<const Tensor*> own;
+    std::vector<Tensor> held;
+    std::vector<c10::Storage> memory;
     std::vector<std::pair<size_t, Tensor>> packed;   // (index, copy)
     std::vector<void*> ptr;
     std::vector<int64_t> numel;
@@ -80,7 +82,23 @@ struct Grads {
     c10::Device device = c10::Device(c10::kCPU);
     int n() const { return (int)ptr.size(); }
     const void* const* cptr() const { return (const void* const*)ptr.data(); }
+    // Before the host waits: other threads of the program run then, and may give the parameters other gradients, or a tensor
+    // other memory.
+    void hold() {
+        held.reserve(own.size());
+        for (const Tensor*& t : own) {
+            held.push_back(*t);
+            memory.push_back(t->storage());
+            t = &held.back();
+        }
+    }
 };
+
+// A number that the device is still computing; other Python threads run while the host waits for it.
+double wait_for(const Tensor& t) {
+    pybind11::gil_scoped_release others;
+    return t.item<double>();
+}
 
 Grads collect(const std::vector<Tensor>& params, const char* what) {
     torch::NoGradGuard no_grad;
@@ -235,9 +253,10 @@ struct Norm {
         check_rc(gso_grad_norm(g.n(), g.cptr(), g.numel.data(), g.type.data(), kind, temp.data_ptr(), bytes, out(), st), what);
     }
     // error_if_nonfinite: the norm before anything changes
-    void look(const Grads& g, int kind, void* st, const char* what) {
+    void look(Grads& g, int kind, void* st, const char* what) {
         form(g, kind, st, what);
-        const float norm = value.item<float>();
+        if (g.held.empty()) g.hold();
+        const double norm = wait_for(value);
         TORCH_CHECK(std::isfinite(norm), what, ": the total norm of the gradients is ", norm,
                     " (error_if_nonfinite); nothing was changed");
     }
@@ -259,7 +278,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& params, double max_norm, double
     const int kind = norm_kind(norm_type, what);
     TORCH_CHECK(max_norm >= 0.0, what, ": max_norm must not be negative or NaN, got ", max_norm);
     check_disjoint(params, what);
-    const Grads g = collect(params, what);
+    Grads g = collect(params, what);
     if (g.own.empty()) return torch::zeros({});
     c10::DeviceGuard guard(g.device);
     if (error_if_nonfinite) check_may_wait(what);
@@ -289,12 +308,13 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
     TORCH_CHECK(exp_avg.size() == n && exp_avg_sq.size() == n && steps.size() == n && scalars.size() == 4 * n &&
                     idle.size() == n, what, ": inconsistent lists");
     // A gradient outlives `parameter.data = other`: the update would read as many elements as the parameter now has.
-    for (size_t i = 0; i < n; ++i) {
-        const Tensor& grad = params[i].grad();
-        TORCH_CHECK(idle[i] || !grad.defined() || grad.sizes() == params[i].sizes(), what, ": a gradient of shape ",
-                    grad.sizes(), " does not have its parameter's shape ", params[i].sizes());
-    }
-    const Grads g = collect(params, what);
+    const auto check_shape = [&](const Tensor& grad, size_t i) {
+        TORCH_CHECK(idle[i] || grad.sizes() == params[i].sizes(), what, ": a gradient of shape ", grad.sizes(),
+                    " does not have its parameter's shape ", params[i].sizes());
+    };
+    for (size_t i = 0; i < n; ++i)
+        if (params[i].grad().defined()) check_shape(params[i].grad(), i);
+    Grads g = collect(params, what);
     TORCH_CHECK(g.own.size() == n, what, ": inconsistent lists");
     if (n == 0) return torch::zeros({});
     torch::NoGradGuard no_grad;
@@ -308,6 +328,15 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
         visible = visibility->element_size() == 1 && !visibility->is_floating_point() ? visibility->contiguous()
                                                                                       : visibility->ne(0).contiguous();
     }
+    // Counts that a checkpoint has brought to the GPU make the host wait, as they do in FusedGaussianAdam.step.  Addresses are
+    // taken behind that.
+    std::vector<double> count(n, 0.0);
+    for (size_t i = 0; i < n; ++i) {
+        TORCH_CHECK(steps[i].numel() == 1, what, ": a step count must be one number");
+        if (idle[i] || visible.defined() || on_host(steps[i])) continue;
+        if (g.held.empty()) g.hold();
+        count[i] = wait_for(steps[i]);
+    }
     std::vector<GsoAdamTensor> table;
     std::vector<Tensor> keep;
     std::vector<size_t> counted;
@@ -319,8 +348,8 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
             TORCH_CHECK(t->device() == dev && t->scalar_type() == torch::kFloat32 && t->is_contiguous() &&
                             t->sizes() == p.sizes(), what,
                         ": parameters and moments must be contiguous float32 tensors of one shape on the gradients' device");
+        check_shape(*g.own[i], i);
         TORCH_CHECK(g.own[i]->scalar_type() == torch::kFloat32, what, ": gradients must be float32");
-        TORCH_CHECK(steps[i].numel() == 1, what, ": a step count must be one number");
         if (idle[i]) continue;
         const int64_t rows = p.dim() > 0 ? p.size(0) : 1;
         TORCH_CHECK(!visible.defined() || visible.numel() == rows, what, ": visibility must have one entry per Gaussian");
@@ -329,8 +358,7 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
         a.lr = s[0]; a.beta1 = s[1]; a.beta2 = s[2]; a.eps = s[3];
         a.bias_correction1 = a.bias_correction2_sqrt = 1.0;
         if (!visible.defined()) {
-            // a count that a checkpoint has brought to the GPU makes the host wait, as it does in FusedGaussianAdam.step
-            const double t = (on_host(steps[i]) ? (double)*steps[i].data_ptr<float>() : steps[i].item<double>()) + 1.0;
+            const double t = (on_host(steps[i]) ? (double)*steps[i].data_ptr<float>() : count[i]) + 1.0;
             a.bias_correction1 = 1.0 - std::pow(a.beta1, t);
             a.bias_correction2_sqrt = std::sqrt(1.0 - std::pow(a.beta2, t));
             counted.push_back(i);
@@ -355,7 +383,12 @@ Tensor clipped_adam(const std::vector<Tensor>& params, const std::vector<Tensor>
     TORCH_CHECK(spans.disjoint(), what, ": a parameter or moment shares memory with another tensor of the step");
     void* st = stream_on(dev);
     Norm r(g);
-    if (error_if_nonfinite) r.look(g, kind, st, what);
+    std::vector<c10::Storage> memory;   // of what the update writes, over the wait
+    if (error_if_nonfinite) {
+        for (size_t i = 0; i < n; ++i)
+            for (const Tensor* t : {&params[i], &exp_avg[i], &exp_avg_sq[i]}) memory.push_back(t->storage());
+        r.look(g, kind, st, what);
+    }
     check_rc(gso_adam_clipped(g.n(), g.cptr(), g.numel.data(), g.type.data(), (int)table.size(), table.data(),
                               visible.defined() ? (const uint8_t*)visible.data_ptr() : nullptr, kind, max_norm,
                               error_if_nonfinite, r.temp.data_ptr(), r.bytes, r.out(), st),

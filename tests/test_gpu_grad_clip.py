@@ -630,3 +630,69 @@ def test_strided_gradients_that_share_memory_are_refused():
     assert abs(float(norm) - ref) <= ref * (U + 1e-11)
     c = 0.1 / (ref + 1e-6)
     assert bool(((wide.double() - keep.double() * c).abs() <= keep.double().abs() * c * 3 * U + SUBNORMAL[torch.float32]).all())
+
+
+def _busy():
+    """Some hundred milliseconds of work in front of whatever the current stream gets next."""
+    a = torch.ones(8192, 8192, device="cuda", dtype=torch.bfloat16)
+    b = torch.empty_like(a)
+    for _ in range(300):
+        torch.mm(a, a, out=b)
+
+
+@pytest.mark.parametrize("call", ["clip", "step", "count"])
+def test_other_python_threads_run_while_the_host_waits(call):
+    """clip and step: for the norm; count: for a step count on the GPU.  What a thread does to `.grad` meanwhile does not
+    reach the call."""
+    import threading
+    import time
+
+    import gsplat_optim as G
+    p, q = (torch.nn.Parameter(torch.ones(5000, 3, device="cuda")) for _ in range(2))
+    opt = G.FusedGaussianAdam([p, q], lr=0.1)
+    for t in (p, q):
+        t.grad = torch.ones_like(t)
+    opt.step()
+    twin = [torch.nn.Parameter(t.detach().clone()) for t in (p, q)]
+    other = G.FusedGaussianAdam(twin, lr=0.1)
+    for t, u in zip((p, q), twin):
+        other.state[u] = {k: v.clone() for k, v in opt.state[t].items()}
+        u.grad = torch.full_like(u, 2.0)
+    if call == "count":
+        for t in (p, q):
+            opt.state[t]["step"] = opt.state[t]["step"].cuda()
+    grads = [torch.full_like(t, 2.0) for t in (p, q)]
+    for t, g in zip((p, q), grads):
+        t.grad = g
+    torch.cuda.synchronize()
+    ticks, stop = [], threading.Event()
+
+    def tick():
+        while not stop.is_set():
+            time.sleep(0.001)
+            ticks.append(time.perf_counter())
+            if len(ticks) > 40:
+                p.grad = q.grad = None
+
+    thread = threading.Thread(target=tick)
+    _busy()
+    thread.start()
+    begin = time.perf_counter()
+    if call == "clip":
+        norm = G.clip_grad_norm_([p, q], 1.0, error_if_nonfinite=True)
+    else:
+        norm = opt.clipped_step(1.0, error_if_nonfinite=call == "step")
+    end = time.perf_counter()
+    stop.set()
+    thread.join()
+    want = G.clip_grad_norm_(twin, 1.0) if call == "clip" else other.clipped_step(1.0)
+    torch.cuda.synchronize()
+    assert end - begin > 0.05, "the call had nothing to wait for"
+    assert sum(begin < t < end for t in ticks) >= 20
+    assert p.grad is None and q.grad is None
+    assert torch.equal(norm, want)
+    if call == "clip":
+        assert all(torch.equal(g, u.grad) for g, u in zip(grads, twin))
+    else:
+        assert all(torch.equal(t, u) for t, u in zip((p, q), twin))
+        assert all(float(opt.state[t]["step"]) == 2.0 for t in (p, q))
