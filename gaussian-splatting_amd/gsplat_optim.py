@@ -456,7 +456,12 @@ def evict_optimizer(optimizer, weights, budget, recent=0, stats=None):
     """`evict_rows` for the whole model: every group's parameter, its optimizer state and the per-Gaussian tensors
     of the dict `stats` keep the chosen rows, and the state moves to the new nn.Parameter as `prune_optimizer` moves
     it.  Returns ({group name: new parameter}, rows, new stats).  Nothing is changed if a tensor does not have one row
-    per weight.  A `ParamGradSink` has to be built anew afterwards, as after densification."""
+    per weight.  A `ParamGradSink` has to be built anew afterwards, as after densification.
+
+    A model that has no more rows than the budget stays as it is: the same parameters with their gradients, the same
+    state and the tensors of `stats` come back, and a sink stays valid (`optimizable[name] is old` tells).  Otherwise
+    the old and the new tensors are alive together until the call returns, so that a failure leaves the old ones: the
+    kept rows of all of them have to fit beside the model."""
     N = weights.numel()
     stats = {} if stats is None else dict(stats)
     moved = []   # (group, [state keys])
@@ -474,6 +479,11 @@ def evict_optimizer(optimizer, weights, budget, recent=0, stats=None):
         tensors.append(p.data)
         tensors += [st[k] for k in keys]
     tensors += list(stats.values())
+    if int(budget) >= N:
+        host = _host()
+        rows = host.evict_select(weights, int(budget), int(recent))
+        host.take_rows(tensors, rows[:0], N)   # refuses what an eviction would refuse
+        return {group["name"]: group["params"][0] for group, _ in moved}, rows, stats
     rows, kept = evict_rows(weights, budget, recent, tensors)
     kept = iter(kept)
     optimizable = {}

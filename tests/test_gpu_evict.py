@@ -471,3 +471,37 @@ def test_c_abi_copies_rows_in_any_order(row_bytes, pitch, order):
     at = rows.long()[:, None] * pitch + torch.arange(row_bytes, device="cuda")[None]
     torch.cuda.synchronize()
     assert torch.equal(dst.view(K, row_bytes), src[at])
+
+
+@pytest.mark.parametrize("over", [0, 7])
+@pytest.mark.parametrize("steps", [0, 2])
+def test_a_model_within_its_budget_stays_as_it_is(steps, over):
+    import gsplat_optim as G
+    N = 3001
+    opt = _optimizer(N, steps)
+    old = {g["name"]: g["params"][0] for g in opt.param_groups}
+    for p in old.values():
+        p.grad = torch.randn_like(p)
+    grads = {k: p.grad for k, p in old.items()}
+    state = {k: dict(opt.state[p]) for k, p in old.items()} if steps else {}
+    values = {k: p.detach().clone() for k, p in old.items()}
+    w = torch.rand(N, device="cuda")
+    stats = dict(weights=w, radii=torch.arange(N, device="cuda", dtype=torch.int32))
+    got, rows, new = G.evict_optimizer(opt, w, N + over, 100, stats)
+    assert rows.dtype == torch.int32 and torch.equal(rows, torch.arange(N, device="cuda", dtype=torch.int32))
+    assert list(got) == list(old) and list(new) == list(stats) and all(new[k] is stats[k] for k in stats)
+    for g in opt.param_groups:
+        k = g["name"]
+        assert got[k] is old[k] and g["params"][0] is old[k] and old[k].grad is grads[k] and torch.equal(old[k], values[k])
+        if steps:
+            assert all(opt.state[old[k]][n] is t for n, t in state[k].items())
+    assert len(opt.state) == (len(old) if steps else 0)
+    opt.step()
+    # what an eviction refuses is refused here too
+    for bad in (torch.rand(N - 1, device="cuda"), torch.rand(N), torch.tensor(1.0, device="cuda")):
+        with pytest.raises(RuntimeError, match="one row per weight"):
+            G.evict_optimizer(opt, w, N + over, 0, dict(bad=bad))
+    with pytest.raises(RuntimeError, match="recent"):
+        G.evict_optimizer(opt, w, N, N + 1)
+    with pytest.raises(RuntimeError, match="float32"):
+        G.evict_optimizer(opt, w.double(), N)
