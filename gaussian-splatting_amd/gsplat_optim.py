@@ -474,6 +474,10 @@ def evict_optimizer(optimizer, weights, budget, recent=0, stats=None):
             raise RuntimeError(f"evict_optimizer: group {group.get('name')!r} has shape {tuple(p.shape)}, the weights "
                                f"have {N} rows")
         st = optimizer.state.get(p, None)
+        for k in ("exp_avg", "exp_avg_sq", "max_exp_avg_sq"):
+            if st and k in st and st[k].shape != p.shape:
+                raise RuntimeError(f"evict_optimizer: {k} of group {group['name']!r} has shape {tuple(st[k].shape)}, its "
+                                   f"parameter {tuple(p.shape)}")
         keys = [k for k, t in st.items() if torch.is_tensor(t) and t.shape == p.shape] if st else []
         moved.append((group, keys))
         tensors.append(p.data)

@@ -156,6 +156,21 @@ def test_shared_memory_is_found_as_by_listing_every_byte():
     assert min(verdicts.count(v) for v in set(verdicts)) > 300 and len(set(verdicts)) == 3
 
 
+@pytest.mark.parametrize("key", ["exp_avg", "exp_avg_sq", "max_exp_avg_sq"])
+def test_eviction_refuses_moments_of_other_rows(key):
+    """They would stay behind, and no longer belong to the rows of their parameter."""
+    import gsplat_optim as G
+    p = _param()
+    opt = torch.optim.Adam([{"params": [p], "name": "xyz"}], amsgrad=True)
+    opt.step()
+    opt.state[p][key] = torch.zeros(5, 3)
+    state = dict(opt.state[p])
+    for budget in (2, 4):
+        with pytest.raises(RuntimeError, match=f"{key} of group 'xyz'"):
+            G.evict_optimizer(opt, torch.ones(4), budget)
+    assert opt.param_groups[0]["params"][0] is p and all(opt.state[p][k] is t for k, t in state.items())
+
+
 def test_c_abi_refuses_bad_arguments():
     from _gsplat_lib import lib
     L = lib()
