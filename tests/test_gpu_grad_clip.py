@@ -696,3 +696,78 @@ def test_other_python_threads_run_while_the_host_waits(call):
     else:
         assert all(torch.equal(t, u) for t, u in zip((p, q), twin))
         assert all(float(opt.state[t]["step"]) == 2.0 for t in (p, q))
+
+
+@pytest.mark.parametrize("norm_type", [2.0, 1.0, math.inf])
+@pytest.mark.parametrize("sizes", [[1000, 3, (20, 7)], [16 * 4096, 1], [16 * 4096 + 1], [300_001, 77, 5000], [9_000_001]],
+                         ids=["small", "17 chunks", "16 chunks and 4 bytes", "joined", "finished"])
+@pytest.mark.parametrize("over", [True, False])
+def test_a_norm_that_was_looked_at_first_clips_to_the_same_bits(sizes, norm_type, over):
+    """The coefficient is 0.3 * norm / (norm + 1e-6), which is 0.3 to 5e-7 for norms of 2 and more; it and the product
+    are rounded to float32 (2 u = 1.2e-7 together), the product once more to the tensor's type."""
+    import gsplat_optim as G
+    one, two = (_make(sizes, [torch.float32, torch.bfloat16, torch.float16], seed=4) for _ in range(2))
+    raw = [g.clone() for g in one]
+    ceiling = _norm64(one, norm_type) * (0.3 if over else 3.0)
+    a = G.clip_grad_norm_(_params(one), ceiling, norm_type)
+    b = G.clip_grad_norm_(_params(two), ceiling, norm_type, error_if_nonfinite=True)
+    assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(one, two))
+    if over:
+        assert not any(torch.equal(x, y) for x, y in zip(two, raw))
+        for x, y in zip(two, raw):
+            c = 0.3   # off by less than 1e-6 in all
+            assert bool(((x.double() - y.double() * c).abs() <= (y.double().abs() * c) * (HALF_STEP[x.dtype] + 1e-6) + SUBNORMAL[x.dtype]).all())
+    else:
+        assert all(torch.equal(x, y) for x, y in zip(two, raw))
+
+
+@pytest.mark.parametrize("N", [300, 4099, 60_000])
+@pytest.mark.parametrize("sparse", [None, 0.3])
+@pytest.mark.parametrize("ceiling", [0.01, 1e9])
+def test_a_norm_that_was_looked_at_first_steps_to_the_same_bits(N, sparse, ceiling):
+    """Moments that are not zero: a first step would be the same for any coefficient."""
+    import gsplat_optim as G
+    a, b, c = (_optimizer(N, G.FusedGaussianAdam, extra=True) for _ in range(3))
+    vis = None if sparse is None else torch.rand(N, device="cuda", generator=torch.Generator(device="cuda").manual_seed(N)) < sparse
+    rows = None if vis is None else N
+    n1 = a.clipped_step(ceiling, vis, rows)
+    n2 = b.clipped_step(ceiling, vis, rows, error_if_nonfinite=True)
+    n3 = G.clip_grad_norm_([g["params"][0] for g in c.param_groups], ceiling, error_if_nonfinite=True)
+    c.step(vis, rows)
+    assert torch.equal(n1, n2) and torch.equal(n1, n3)
+    for x, y, z in zip(_dump(a), _dump(b), _dump(c)):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+@pytest.mark.parametrize("tensors", [40, 41, 90])
+@pytest.mark.parametrize("sparse", [None, 0.0, 0.3])
+@pytest.mark.parametrize("ceiling", [0.01, 1e9])
+def test_a_step_of_more_tensors_than_a_launch_takes(tensors, sparse, ceiling):
+    import gsplat_optim as G
+    N = 700
+
+    def make():
+        gen = torch.Generator().manual_seed(tensors)
+        shapes = [(N, 1 + 5 * k % 23) if sparse is not None else ((k * 977) % 5003 + 1,) if k % 3 else (N, 1 + k) for k in range(tensors)]
+        opt = G.FusedGaussianAdam([{"params": [torch.nn.Parameter(torch.randn(*s, generator=gen).cuda())], "lr": 10.0 ** -(1 + k % 4),
+                                    "betas": (0.8 + 0.002 * k, 0.99)} for k, s in enumerate(shapes)], eps=1e-15)
+        for _ in range(2):
+            _fill(opt, gen)
+            opt.step()
+        _fill(opt, gen)
+        return opt
+
+    a, b = make(), make()
+    before = _dump(a)
+    vis = None if sparse is None else torch.rand(N, device="cuda", generator=torch.Generator(device="cuda").manual_seed(N)) < sparse
+    rows = None if vis is None else N
+    for known in (False, True):
+        n1 = G.clip_grad_norm_([g["params"][0] for g in b.param_groups], ceiling)
+        b.step(vis, rows)
+        n2 = a.clipped_step(ceiling, vis, rows, error_if_nonfinite=known)
+        assert torch.equal(n1, n2)
+        assert all(torch.equal(x, y) for x, y in zip(_dump(a), _dump(b)))
+        for ga, gb in zip(a.param_groups, b.param_groups):
+            gb["params"][0].grad = ga["params"][0].grad.clone()
+    for x, y, k in zip(_dump(a)[::4], before[::4], range(tensors)):
+        assert torch.equal(x, y) == (sparse == 0.0), k
