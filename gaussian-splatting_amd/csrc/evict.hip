@@ -1,11 +1,18 @@
-// Keeping a model within a row budget.  Alpha compositing is attention: along a
-// ray the Gaussians' weights are non-negative and sum to at most one, and a
-// view's forward returns their sums per Gaussian.  The rows of the parameters
+// Keeping a model within a row budget.  Alpha compositing is attention: a
+// pixel's weights alpha * T over the Gaussians of its ray are non-negative and
+// sum to at most one; their sums over a view's pixels are the gradient of the
+// image with respect to the Gaussians' colours.  The rows of the parameters
 // and of the optimizer state are the cache that these weights read, new rows
 // are appended at its end, and eviction keeps the newest rows and the heaviest
 // of the others:
 //
-//   w_i <- decay * w_i + sigmoid(o_i) * sum over views of contribution_v[i]
+//   w_i <- decay * w_i + s_i * sum over views of contribution_v[i]
+//
+// with s = 1 for contributions that are weights.  With s = sigmoid(opacity) and
+// the forward's gauss_sum (T over the pixels that test the Gaussian, whatever
+// its alpha there) the sum is an upper bound of the weight, and no more: it
+// overrates splats that are small against a tile.
+//
 //   keep = { i >= N - recent }  and the (budget - recent) first of the others
 //          in the order (larger weight, then lower index), a NaN last
 //

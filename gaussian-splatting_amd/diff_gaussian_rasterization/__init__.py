@@ -465,3 +465,28 @@ class GaussianRasterizer(nn.Module):
         reps = torch.Tensor([]) if reps is None else reps
         return _RasterizeGaussiansParams.apply(xyz, means2D, features_dc, features_rest, opacity, scaling, rotation,
                                                self.raster_settings, reps, grad_sink)
+
+    @torch.no_grad()
+    def blending_weights(self, xyz, opacity, scaling, rotation):
+        """What each Gaussian contributes to this view: its weights alpha * T summed over the pixels that blend it, [P],
+        from the model's raw parameters (as `forward_params` takes them).  A pixel's weights are non-negative and sum
+        to at most one; a Gaussian that no pixel blends has zero.
+
+        The image is linear in the Gaussians' colours with these weights as coefficients, so they are the gradient of
+        the sum of one colour channel with respect to the Gaussians' values in it: one forward and one backward of
+        the view.  (`gauss_sum` is another quantity: T, without alpha, over all pixels that test the Gaussian.)"""
+        rs = self.raster_settings
+        empty = torch.Tensor([])
+        colors = torch.zeros_like(xyz)
+        opacity, scales, rotations = torch.sigmoid(opacity), torch.exp(scaling), nn.functional.normalize(rotation)
+        (num_rendered, color, radii, geomBuffer, binningBuffer, imgBuffer, *_) = _C.rasterize_gaussians(
+            rs.bg, xyz, colors, opacity, scales, rotations, rs.scale_modifier, empty, rs.viewmatrix, rs.projmatrix,
+            rs.tanfovx, rs.tanfovy, rs.image_height, rs.image_width, empty, rs.sh_degree, rs.campos, rs.prefiltered,
+            rs.antialiasing, rs.debug, empty)
+        grad_color = torch.zeros_like(color)
+        grad_color[0] = 1.0
+        grads = _C.rasterize_gaussians_backward(
+            rs.bg, xyz, radii, colors, opacity, scales, rotations, rs.scale_modifier, empty, rs.viewmatrix, rs.projmatrix,
+            rs.tanfovx, rs.tanfovy, grad_color, empty, empty, empty, rs.sh_degree, rs.campos, geomBuffer, num_rendered,
+            binningBuffer, imgBuffer, rs.antialiasing, rs.debug, empty)
+        return grads[1][:, 0].contiguous()

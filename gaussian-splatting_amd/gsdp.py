@@ -202,8 +202,7 @@ def reduce_densify_stats(xyz_gradient_accum, denom, max_radii2D, group=None):
 
 
 def reduce_weights(weights, group=None):
-    """The blending weights that the ranks accumulated from their own views (`gsplat_optim.accumulate_weights`),
-    summed, as a new tensor: what every rank hands to `gsplat_optim.evict_optimizer`, so that all replicas keep the same
+    """The weights that the ranks accumulated from their own views (`gsplat_optim.accumulate_weights`), summed, as a new tensor: what every rank hands to `gsplat_optim.evict_optimizer`, so that all replicas keep the same
     rows.  The ranks' own weights stay as they are and can be added to further; the eviction then filters them."""
     total = weights.clone()
     if dist.is_initialized() and dist.get_world_size(group) > 1:

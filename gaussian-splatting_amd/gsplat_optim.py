@@ -428,11 +428,15 @@ def accumulate_weights(weights, contributions, opacity=None, decay=1.0):
 
         weights = decay * weights + sigmoid(opacity) * (contributions[0] + contributions[1] + ...)
 
-    `contributions`: a list of [N] tensors, or one: the `gauss_sum` of each rendered view (the transmittance that
-    reached the Gaussian, summed over its pixels); times the opacity it is what the Gaussian could add to the images, as
-    attention weights summed over queries are what a cache entry gave.  `opacity`: the raw opacities ([N] or [N, 1],
-    logits), None for contributions that are weights already.  decay < 1 forgets old views.  All float32 on one
-    GPU.  With several ranks each accumulates its own views: see `gsdp.reduce_weights`."""
+    `contributions`: a list of [N] tensors, or one.  With opacity=None they are weights as they are: the views'
+    `GaussianRasterizer.blending_weights`, what each Gaussian contributed to the images, as attention weights summed over
+    queries are what a cache entry gave.  With the raw opacities ([N] or [N, 1], logits) they are what is to be
+    multiplied by the activated ones: the `gauss_sum` of each rendered view, which costs no rendering of its own, but
+    counts the transmittance of every pixel that tests the Gaussian, whatever its alpha there.  The product is an
+    upper bound of the blending weight (in free space some six times it for round splats much larger than a tile, whose
+    bounding square is tested, and a hundred times and more for those below a pixel), so it ranks Gaussians of
+    different sizes differently.  decay < 1 forgets old views.  All float32 on one GPU.  With several ranks each
+    accumulates its own views: see `gsdp.reduce_weights`."""
     contributions = [contributions] if isinstance(contributions, torch.Tensor) else list(contributions)
     _host().accumulate_weights(weights, contributions, opacity, float(decay))
     return weights

@@ -485,11 +485,14 @@ int gso_adam_clipped(int ngrads, const void* const* grads, const int64_t* numels
                      const GsoAdamTensor* tensors, const uint8_t* visible, int norm_type, double max_norm, int norm_known,
                      void* temp, size_t temp_bytes, float* norm, void* stream);
 
-/* A model within a row budget: the views' blending weights are accumulated per Gaussian, and the lightest rows go.
+/* A model within a row budget: what the views say is accumulated per Gaussian, and the lightest rows go.
  * No counterpart in the reference, whose model only shrinks by opacity and size (scene/gaussian_model.py:237-247).
  *   gso_accumulate_weights: weights[i] = decay * weights[i] + s_i * (contributions[0][i] + ... ), in place;
- *     contributions: HOST array of `views` device pointers to [N] floats (a view's gauss_sum); s_i =
- *     sigmoid(opacity[i]) of the raw opacities, or 1 when opacity is NULL.
+ *     contributions: HOST array of `views` device pointers to [N] floats; s_i = sigmoid(opacity[i]) of the raw
+ *     opacities, or 1 when opacity is NULL.  A view's blending weights, the sums of alpha * T, are the gradient of the
+ *     sum of one colour channel with respect to the Gaussians' colours (dL_dcolors where dL_dout_color is 1 in that
+ *     channel); with opacity NULL they accumulate as they are.  gauss_sum with the opacities gives an upper bound of
+ *     them only (T of every pixel that tests the Gaussian, whatever its alpha there).
  *   gso_evict_select: rows (device, min(N, budget) ints) = in ascending order the last `recent` rows (all N when
  *     recent >= N) and, of the others, the budget - recent of largest weight; of equal weights the lower index is
  *     kept, -0 equals 0, and a NaN lies below everything.  0 <= recent <= budget, N < 2^31.

@@ -34,6 +34,14 @@ def test_there_is_no_cpu_path():
     assert torch.equal(p.grad, torch.ones(4, 3)) and torch.equal(p.detach(), torch.ones(4, 3))
 
 
+def test_blending_weights_need_a_gpu():
+    from diff_gaussian_rasterization import GaussianRasterizationSettings, GaussianRasterizer
+    z = torch.zeros
+    rs = GaussianRasterizationSettings(8, 8, 1.0, 1.0, z(3), 1.0, torch.eye(4), torch.eye(4), 0, z(3), False, False, False)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        GaussianRasterizer(rs).blending_weights(z(4, 3), z(4, 1), z(4, 3), z(4, 4))
+
+
 def test_arguments_are_checked_before_anything_runs():
     import gsplat_optim as G
     p = _param()
