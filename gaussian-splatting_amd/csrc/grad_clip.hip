@@ -7,8 +7,9 @@
 // Nothing here has a counterpart in the reference, which never bounds its
 // gradients.  A launch takes a table of tensors by value (no copy to the
 // device, so it can be captured into a graph); the tensors are cut into
-// chunks, a workgroup sums every 2048th chunk, and the workgroups' sums are
-// added in a fixed order: the norm is the same bits in every run.
+// chunks, each of n <= 2048 workgroups sums every n-th chunk, and the
+// workgroups' sums are added in a fixed order: the norm is the same bits in
+// every run.
 // Sums are held in 64 bits: squares of float32 values neither overflow nor
 // vanish there.
 #include "kernels.h"
@@ -19,7 +20,7 @@ namespace gs {
 
 constexpr int NORM_THREADS = 256;
 constexpr int NORM_TABLE = 240;     // tensors per launch of the norm and scale kernels (kernel arguments: 3.9 KB)
-constexpr int NORM_GROUPS = 2048;   // workgroups of the norm kernel: eight per CU
+constexpr int NORM_GROUPS = 2048;   // workgroups of the norm kernel at most: eight per CU
 constexpr int ADAM_TABLE = 40;      // tensors per launch of the Adam kernel
 constexpr int CHUNK_BYTES = 16384;  // a chunk of a tensor, from its start rounded down to 16 bytes: four vectors a thread
 constexpr int ADAM_CHUNK = 2048;    // elements of a workgroup of the dense Adam kernel: two vectors a thread
@@ -263,9 +264,11 @@ __device__ __forceinline__ void scale_chunk(const Chunk& c, int tid, float s) {
     });
 }
 
-// ONCE: the gradients are not read again through the caches' help (a norm alone, or an Adam step, whose other six
-// streams push them out): non-temporal loads, 7.0 TB/s on 1.5 GB where ordinary ones reach 6.2.  A clip reads them
-// again at once; ordinary loads leave up to 256 MB in the last-level cache for it.
+// ONCE: non-temporal loads, for a norm alone and before an Adam step: 7.0 TB/s on 1.5 GB where ordinary ones reach 6.2.
+// A clip reads the gradients again at once; ordinary loads leave up to 256 MB in the last-level cache for it.  Before a
+// step, with / without (us): sparse, a tenth visible, 1 M Gaussians (252 MB) 174 / 182, 6 M (1.5 GB) 950 / 990, 0.3 M 57
+// either way; dense, 0.1 M (25 MB) 41.5 / 39.4, 0.3 M 110 / 100, 1 M 343 / 308, 2.5 M 870 / 832, 6 M 2118 / 2104: a dense
+// step finds part of its gradients in the cache after ordinary loads, which this rule does not use.
 template <int KIND, bool ONCE>
 __global__ void __launch_bounds__(NORM_THREADS) norm_kernel(const NormTable t, uint64_t* __restrict__ partial) {
     typedef Share<KIND> S;
@@ -485,7 +488,7 @@ __global__ void __launch_bounds__(NORM_THREADS) adam_clipped_sparse_kernel(const
         }
     }
     __syncthreads();
-    const uint32_t total = s_count * W;   // less than SPARSE_CHUNK, or one row
+    const uint32_t total = s_count * W;   // at most SPARSE_CHUNK, or one row
     // x / W by one multiplication: x and W stay below 2^13 unless the row is the only one
     const uint32_t magic = W > 1 && W < SPARSE_CHUNK ? 0xffffffffu / W + 1 : 0;
     float *p = e.param + row0 * W, *m = e.exp_avg + row0 * W, *v = e.exp_avg_sq + row0 * W;
@@ -602,7 +605,7 @@ static hipError_t launch_norm_for(NormUse use, int n, const void* const* grads, 
             else launch_small<0>(t, use == NORM_CLIP, max_norm, r, norm, st);
             return;
         }
-        const uint32_t rounds = (t.chunks + NORM_GROUPS - 1) / NORM_GROUPS;   // the same number for every workgroup
+        const uint32_t rounds = (t.chunks + NORM_GROUPS - 1) / NORM_GROUPS;   // of every workgroup; some take one chunk less
         const unsigned groups = (t.chunks + rounds - 1) / rounds;
         uint64_t* p = norm_partials(temp) + count;
         if (kind == 2) launch_norm<2>(t, use == NORM_CLIP, groups, p, st);

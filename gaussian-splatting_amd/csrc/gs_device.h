@@ -187,7 +187,7 @@ __device__ __forceinline__ float select_or_zero(uint64_t m, float v) {
     return r;
 }
 
-// splat_power() with its two squared terms as one packed multiply each; same operation
+// splat_power() with its two squared terms side by side; same operation
 // order per term, hence the same roundings.  xy: centre, pix: pixel, cxz: (conic.x, conic.z).
 __device__ __forceinline__ float splat_power_pk(f2 xy, f2 pix, f2 cxz, float cy, f2* d) {
     *d = xy - pix;

@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(TILE_PIX) __attribute__((amdgpu_waves_per_eu(D
 render_fwd_kernel(const RenderFwdArgs a) {
     constexpr int XQ = DIM > 4 ? (DIM - 4) / 4 : 0;   // extra 16-byte pieces of a feature row
     // One SplatRec per instance, regrouped: the test of an instance needs the first two
-    // quarters only, the other two feed packed (two-float) multiply-adds as they are.
+    // quarters only, the other two feed the multiply-adds of channel pairs as they are.
     __shared__ float4 s_q[4][TILE_PIX];
     float4* const s_q0 = s_q[0];  // x, y, -conic.x / 2, -conic.z / 2 (see splat_power_prescaled)
     float4* const s_q1 = s_q[1];  // conic.y, tau, opacity, Gaussian index (bits)
@@ -208,9 +208,9 @@ render_fwd_kernel(const RenderFwdArgs a) {
                                  : "memory");
                 if (lane_in(bm)) {
                     // forward.cu:454-464: C += c * alpha * T per channel.  The weight alpha * T is formed
-                    // once and each pair of channels is one packed fused multiply-add (the sums are
-                    // compared at 1e-5 absolute, no integer output depends on them): 5 instructions where
-                    // the reference's order of operations takes 12.
+                    // once and each channel is one fused multiply-add (the sums are compared at 1e-5
+                    // absolute, no integer output depends on them): 9 instructions for the eight channels
+                    // of DIM = 4 where the reference's order of operations takes 24.
                     const float wgt = alpha * T;
                     const f2 w2 = {wgt, wgt};
                     Crg = __builtin_elementwise_fma((f2){q2.x, q2.y}, w2, Crg);

@@ -458,8 +458,9 @@ int gso_gather_rows(const void* src, void* dst, const uint32_t* src_of_dst, int6
  * allowed, the pointer is then ignored) and of GsoTypes; a tensor's elements are contiguous, tensors may be of different
  * types.  `temp`: device, 8-byte aligned, gso_norm_temp_bytes(n) bytes.
  *   gso_grad_norm: *norm (device, float32); also left in `temp`.
- *   gso_clip_grads: *norm, then g <- g * c in place, each product rounded once to the tensor's type; with c = 1
- *     nothing is written.  No two tensors may share memory.
+ *   gso_clip_grads: *norm, then g <- g * c in place, each product formed in float32 and rounded from there to the
+ *     tensor's type (two roundings for bfloat16 and float16); with c = 1 nothing is written.  No two tensors may share
+ *     memory.
  *   gso_adam_clipped: *norm of the `ngrads` gradients, then Adam's update of the `n` tensors with the gradient c * g (the
  *     product rounded to float32, as clipping in place would store it; the gradients keep their values), operation by
  *     operation gso_adam_update's.  `visible`: device bytes, one per row, or NULL; applies to every tensor.
