@@ -19,6 +19,7 @@ diff_gaussian_rasterization: the reference switches its renderer to a branch
 that does not work with the fork's rasterizer as soon as that import succeeds
 (train.py:38-42, gaussian_renderer/__init__.py:138-150).
 """
+import contextlib
 import ctypes as C
 import math
 
@@ -44,46 +45,55 @@ class FusedGaussianAdam(torch.optim.Adam):
             # a row is visible where the mask is not zero, whatever its type (radii, weights)
             vis = visibility if visibility.dtype in (torch.bool, torch.uint8) else visibility != 0
             vis = vis.contiguous().view(torch.uint8)
-        for group in self.param_groups:
-            beta1, beta2 = group["betas"]
-            lr, eps = float(group["lr"]), float(group["eps"])
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
-                if p.grad.shape != p.shape:   # a gradient outlives `p.data = other`
-                    raise RuntimeError(f"FusedGaussianAdam: a gradient of shape {tuple(p.grad.shape)} does not have its "
-                                       f"parameter's shape {tuple(p.shape)}")
-                if vis is not None and vis.device != p.device:
-                    raise RuntimeError(f"FusedGaussianAdam: visibility must be on {p.device}, got {vis.device}")
-                if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
-                    raise RuntimeError("FusedGaussianAdam needs contiguous float32 GPU parameters (there is no CPU path)")
-                g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
-                st = self.state[p]
-                if len(st) == 0:
-                    st["step"] = torch.tensor(0.0, dtype=torch.float32)
-                    st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                    st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                for t in (g, st["exp_avg"], st["exp_avg_sq"]):
-                    if t.shape != p.shape or t.dtype != torch.float32 or t.device != p.device or not t.is_contiguous():
-                        raise RuntimeError("FusedGaussianAdam: gradient and moments must be contiguous float32 tensors of the "
-                                           f"parameter's shape {tuple(p.shape)} on {p.device}, got {tuple(t.shape)} {t.dtype} "
-                                           f"on {t.device}")
-                rows = p.shape[0] if p.dim() > 0 else 1
-                width = p.numel() // max(rows, 1)
-                if vis is not None:
-                    if N is not None and rows != N:
-                        continue   # a group that is not per-Gaussian takes no sparse step
-                    if vis.numel() != rows:
-                        raise RuntimeError("visibility must have one entry per Gaussian")
-                    bc1, bc2s = 1.0, 1.0
-                else:
-                    st["step"] += 1
-                    t = float(st["step"])
-                    bc1, bc2s = 1.0 - beta1 ** t, math.sqrt(1.0 - beta2 ** t)
-                with torch.cuda.device(p.device):
-                    check(L.gso_adam_update(p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(),
-                                            st["exp_avg_sq"].data_ptr(), None if vis is None else vis.data_ptr(),
-                                            rows, width, lr, beta1, beta2, eps, bc1, bc2s, stream_of(p.device)),
+        current = None   # the device whose context is entered: once for all tensors where they are on one
+        with contextlib.ExitStack() as contexts:
+            for group in self.param_groups:
+                beta1, beta2 = group["betas"]
+                lr, eps = float(group["lr"]), float(group["eps"])
+                for p in group["params"]:
+                    g = p.grad
+                    if g is None:
+                        continue
+                    shape, dev = p.shape, p.device
+                    rows = shape[0] if shape else 1
+                    # a group that is not per-Gaussian takes no sparse step
+                    idle = vis is not None and N is not None and rows != N
+                    if not idle and g.shape != shape:   # a gradient outlives `p.data = other`
+                        raise RuntimeError(f"FusedGaussianAdam: a gradient of shape {tuple(g.shape)} does not have its "
+                                           f"parameter's shape {tuple(shape)}")
+                    if not idle and vis is not None and vis.device != dev:
+                        raise RuntimeError(f"FusedGaussianAdam: visibility must be on {dev}, got {vis.device}")
+                    if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
+                        raise RuntimeError("FusedGaussianAdam needs contiguous float32 GPU parameters (there is no CPU path)")
+                    st = self.state[p]
+                    if len(st) == 0:
+                        st["step"] = torch.tensor(0.0, dtype=torch.float32)
+                        st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                        st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                    if idle:
+                        continue
+                    g = g if g.is_contiguous() else g.contiguous()
+                    m, v = st["exp_avg"], st["exp_avg_sq"]
+                    for t in (g, m, v):
+                        if t.dtype is not torch.float32 or t.device != dev or t.shape != shape or not t.is_contiguous():
+                            raise RuntimeError("FusedGaussianAdam: gradient and moments must be contiguous float32 tensors of "
+                                               f"the parameter's shape {tuple(shape)} on {dev}, got {tuple(t.shape)} "
+                                               f"{t.dtype} on {t.device}")
+                    width = p.numel() // max(rows, 1)
+                    if vis is not None:
+                        if vis.numel() != rows:
+                            raise RuntimeError("visibility must have one entry per Gaussian")
+                        bc1, bc2s = 1.0, 1.0
+                    else:
+                        st["step"] += 1
+                        t = float(st["step"])
+                        bc1, bc2s = 1.0 - beta1 ** t, math.sqrt(1.0 - beta2 ** t)
+                    if dev != current:
+                        contexts.enter_context(torch.cuda.device(dev))
+                        current = dev
+                    check(L.gso_adam_update(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(),
+                                            None if vis is None else vis.data_ptr(), rows, width, lr, beta1, beta2, eps, bc1,
+                                            bc2s, stream_of(dev)),
                           "adam update")
         return loss
 

@@ -386,3 +386,14 @@ def test_a_sparse_step_with_visibility_in_host_memory_is_refused():
     assert len(opt.state) == 0 and bool((p == 1).all())
     opt.step(torch.ones(100, dtype=torch.bool, device="cuda:0"), 100)
     assert bool((p < 1).all())
+
+
+def test_a_group_that_takes_no_sparse_step_is_left_alone():
+    """Whatever its gradient is: it is not read."""
+    from gsplat_optim import FusedGaussianAdam
+    p, q = torch.nn.Parameter(torch.ones(100, 3, device="cuda:0")), torch.nn.Parameter(torch.ones(7, 3, device="cuda:0"))
+    opt = FusedGaussianAdam([p, q], lr=0.1)
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    q.data = torch.ones(9, 3, device="cuda:0")     # the gradient keeps its seven rows
+    opt.step(torch.ones(100, dtype=torch.bool, device="cuda:0"), 100)
+    assert bool((p < 1).all()) and bool((q == 1).all()) and q.shape == (9, 3)
